@@ -3,7 +3,6 @@ distillation from a teacher's top log probabilities, each with its gradient.
 
 Every case is one call of a public entry point of ``vitm_amd`` (``own``) or the same operator in elementary torch
 operations in 32 bits, rounded once at the end.  ``exact`` holds the definitions in 64 bits."""
-import functools
 import math
 import os
 import sys
@@ -123,15 +122,11 @@ def prepare(case, seed):
         idx[:, -1] = torch.where(short, torch.full_like(labels, -1), idx[:, -1])
     s["indices"] = idx
     s["logits"] = z.to(_dtype(case))
-    if own:                                                     # the loss object is made once by a program
-        s["loss"] = _package()[1].DistillationLoss(temperature=case["temperature"], label_weight=case["label_weight"],
-                                                   tail=case["tail"], reduction="none" if case["mode"] == "loss" else "mean")
     s["labels"] = torch.where(dropped, torch.full_like(labels, IGNORE), labels)
     return s
 
 
 # ---- the framework's calls --------------------------------------------------------------------------------------
-@functools.lru_cache(maxsize=None)
 def _package():
     here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "vision-transformer_amd")
     if here not in sys.path:
@@ -142,7 +137,7 @@ def _package():
 
 
 def _run_own(s):
-    vitm = _package()[0]
+    vitm, training = _package()
     c = s["case"]
     if c["op"] == "log_probs":
         z = s["logits"]
@@ -163,7 +158,8 @@ def _run_own(s):
             (out["dlogits"],) = torch.autograd.grad(heads, z, ups)
             out = {k: v.detach() for k, v in out.items()}
         return out
-    loss_fn = s["loss"]
+    loss_fn = training.DistillationLoss(temperature=c["temperature"], label_weight=c["label_weight"], tail=c["tail"],
+                                        reduction="none" if c["mode"] == "loss" else "mean")
     args = (s["teacher"], s["indices"], s["labels"])
     if c["mode"] == "fused":
         loss, dz = loss_fn.loss_and_grad(s["logits"], *args)
