@@ -206,6 +206,13 @@ __device__ __forceinline__ void barrier_after_stores() {
   __syncthreads();
 }
 
+// What lanes of this wave wrote to LDS before is seen by its other lanes behind it.  LDS serves a wave's accesses in order, so this
+// costs no instruction; without it nothing keeps the compiler from moving a read in front of the write.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // ---- reductions over a workgroup of G threads --------------------------------------------------------------------
 // Within a wave by lane permutations of the VALU (DPP): a shuffle through LDS takes tens of cycles of a pipe that all waves of a
 // CU share, and the short rows of a classifier are mostly such reductions.  All lanes have to be active.
@@ -965,6 +972,7 @@ template <typename T> __device__ __forceinline__ void read_list(const DistillArg
 __device__ __forceinline__ void finish_row(const DistillArgs& A, int r, Sums dn, ListScratch& L) {
   const int lane = threadIdx.x & 63;
   const float T_ = A.temperature, inv_t = 1.f / T_, cT = inv_t * kLog2e, c1 = kLog2e, a = A.label_weight;
+  wave_sync();   // read_list's, where one wave has the row and met no barrier since
   const float z[2] = {L.z[lane], L.z[lane + 64]}, q[2] = {L.q[lane], L.q[lane + 64]};
   float q_rest = L.q_rest, Q = L.Q, tail_loss = 0.f;
   if (dn.m == NINF && dn.s == 0.f) q_rest = 0.f;   // no class outside the list: no tail term
