@@ -690,3 +690,22 @@ def test_graphed_step_refuses_a_teacher_that_changed():
     with pytest.raises(RuntimeError, match="teacher's weights"):
         g.step(x, y)
     assert all(torch.equal(a, b) for a, b in zip(before, m.parameters()))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_gradient_interleaved_with_the_logits(dtype):
+    """Rows of logits and gradient in turn, in one buffer: their spans meet, the rows do not."""
+    from vitm_amd import _lib
+    lib = _lib.load()
+    R, V, K = 5, 1001, 3
+    buf = torch.zeros(R, 2 * V, device=DEV, dtype=dtype)
+    z, out = buf[:, :V], buf[:, V:]
+    z.copy_(_scores(R, V, dtype, 3))
+    kept = z.clone()
+    tl, idx = _teacher(R, V, K, 3)
+    row_loss = torch.empty(R, device=DEV)
+    _lib.check(lib.vitm_distill(z.data_ptr(), _lib.BF16 if dtype == BF else _lib.F32, 0, 2 * V, R, R, V, 1.0, 0.0, 1, tl.data_ptr(),
+                                idx.data_ptr(), K, None, -100, 0, row_loss.data_ptr(), None, None, None, out.data_ptr(), 0, 2 * V,
+                                torch.cuda.current_stream().cuda_stream), "distill")
+    assert torch.equal(z, kept)
+    _check_distill(z, tl, idx, None, row_loss, out, 1.0, 0.0, True)

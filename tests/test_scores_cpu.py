@@ -247,3 +247,29 @@ def test_oracle_gradients_are_differences():
             _, _, dz, _ = O.distill(z, tl, idx, lab, T, a, tail)
             d = diff(lambda z: O.distill(z, tl, idx, lab, T, a, tail)[0].sum())
             assert (dz - d).abs().max() < 1e-8, (tail, a)
+
+
+def test_c_abi_refuses_a_gradient_that_meets_the_logits():
+    """Shifted by a class, from in front or behind, or with another pitch, not only at the same address; rows that lie next to the
+    others, as in an interleaved buffer, are not a meeting (test_gpu_scores.py runs them)."""
+    from vitm_amd import _lib
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(1 << 16)
+    at = lambda floats: ctypes.c_void_p(((ctypes.addressof(buf) + 255) & ~255) + 4 * floats)
+    p, f, V, R = at(8192), ctypes.c_float, 9, 6
+
+    def all_refuse(z, ld_outer, ld, inner, dz, ldd_outer, ldd):
+        rows = (z, 1, ld_outer, ld, inner, R, V, f(1.0))
+        for call, args in ((lib.vitm_log_probs_bwd, (p, 1, -100, p, 2, p, p, p, p, p, p)),
+                           (lib.vitm_distill, (f(0.0), 0, p, p, 4, p, -100, 1, p, p, p, p)),
+                           (lib.vitm_distill_bwd, (f(0.0), 0, p, p, 4, p, -100, 1, p, p, p))):
+            rc = call(*rows, *args, dz, ldd_outer, ldd, None)
+            assert rc == -1 and b"same memory" in lib.vitm_last_error(), (rc, lib.vitm_last_error())
+
+    all_refuse(at(0), 0, 9, R, at(1), 0, 9)
+    all_refuse(at(53), 0, 9, R, at(0), 0, 9)           # the last class of the last row
+    all_refuse(at(0), 0, 20, R, at(8), 0, 20)
+    all_refuse(at(12), 0, 20, R, at(0), 0, 20)         # the end of a row in the next one's start
+    all_refuse(at(0), 0, 0, R, at(4), 0, 9)            # one row of logits, repeated
+    all_refuse(at(0), 100, 10, 3, at(35), 60, 11)      # two strides
+    all_refuse(at(85), 9, 1, 3, at(0), 60, 11)

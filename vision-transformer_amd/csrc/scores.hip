@@ -1364,6 +1364,27 @@ int check_out(const char* what, const void* out, int dtype, int64_t ld_outer, in
   VITM_REQUIRE((in == 1 || ld >= V) && (inner >= R || ld_outer >= (in - 1) * ld + V), "%s: rows of the gradient overlap", what);
   return VITM_OK;
 }
+// Whether a row of the gradient and a row of the logits share memory.  The gradient's rows are apart and in ascending order
+// (check_out), so a row of the logits meets one of them if it meets the last that starts in front of its own end.  Row by row only
+// where the two spans meet at all, as of a gradient interleaved with the logits.
+bool rows_meet(const void* logits, const void* out, int dtype, const RowsAt& at, const RowsAt& out_at, int R, int V) {
+  const int64_t es = dtype == VITM_BF16 ? 2 : 4;
+  const int in = at.inner < R ? at.inner : R, blocks = (R - 1) / in + 1;
+  const int64_t span = (blocks - 1) * at.ld_outer + (in - 1) * at.ld + V, out_span = out_at.offset(R - 1) + V;
+  const int64_t d = ((intptr_t)logits - (intptr_t)out) / es;   // of the first rows
+  if (d >= out_span || d + span <= 0) return false;
+  for (int r = 0; r < R; ++r) {
+    const int64_t a = d + at.offset(r), last = a + V - 1;   // the row's classes, from the gradient's first
+    if (last < 0) continue;
+    int64_t o = blocks == 1 ? 0 : last / out_at.ld_outer;
+    o = o < blocks - 1 ? o : blocks - 1;
+    const int64_t in_block = R - o * in < in ? R - o * in : in;
+    int64_t i = in == 1 ? 0 : (last - o * out_at.ld_outer) / out_at.ld;
+    i = i < in_block - 1 ? i : in_block - 1;
+    if (o * out_at.ld_outer + i * out_at.ld + V > a) return true;
+  }
+  return false;
+}
 constexpr float kMinTemperature = 1e-6f, kMaxTemperature = 1e6f;
 int check_temperature(const char* what, float t) {
   VITM_REQUIRE(t >= kMinTemperature && t <= kMaxTemperature, "%s: temperature %g, supported are %g to %g", what, (double)t,
@@ -1507,7 +1528,8 @@ extern "C" int vitm_log_probs_bwd(const void* logits, int dtype, int64_t ld_oute
   VITM_REQUIRE(!g_logprobs || targets, "vitm_log_probs_bwd: null pointer");
   VITM_REQUIRE(!g_top || top_indices, "vitm_log_probs_bwd: null pointer");
   VITM_REQUIRE(!g_entropy || entropy, "vitm_log_probs_bwd: null pointer");
-  VITM_REQUIRE(dlogits != logits, "vitm_log_probs_bwd: logits and gradient in the same memory");
+  VITM_REQUIRE(!rows_meet(logits, dlogits, dtype, {ld_outer, ld, inner}, {ldd_outer, ldd, inner}, R, V),
+               "vitm_log_probs_bwd: logits and gradient in the same memory");
   const Cut C = cut_rows(R, row_granules(dtype, V, slack_of(logits, dtype, ld_outer, ld, inner, R)));
   if (check_grid("vitm_log_probs_bwd", R, C.nseg, C.G) != VITM_OK) return VITM_EINVAL;
   LogProbsBwdArgs A = {};
@@ -1567,7 +1589,8 @@ extern "C" int vitm_distill(const void* logits, int dtype, int64_t ld_outer, int
   if (dlogits) {
     const int rd = check_out("vitm_distill", dlogits, dtype, ldd_outer, ldd, inner, R, V);
     if (rd != VITM_OK) return rd;
-    VITM_REQUIRE(dlogits != logits, "vitm_distill: logits and gradient in the same memory");
+    VITM_REQUIRE(!rows_meet(logits, dlogits, dtype, {ld_outer, ld, inner}, {ldd_outer, ldd, inner}, R, V),
+                 "vitm_distill: logits and gradient in the same memory");
   }
   const int nq = row_granules(dtype, V, slack_of(logits, dtype, ld_outer, ld, inner, R));
   if (check_grid("vitm_distill", R, 1, 1024) != VITM_OK) return VITM_EINVAL;
@@ -1610,7 +1633,8 @@ extern "C" int vitm_distill_bwd(const void* logits, int dtype, int64_t ld_outer,
   VITM_REQUIRE(state && upstream, "vitm_distill_bwd: null pointer");
   VITM_REQUIRE(reduction >= VITM_REDUCE_NONE && reduction <= VITM_REDUCE_SUM, "vitm_distill_bwd: unknown reduction %d", reduction);
   VITM_REQUIRE(reduction != VITM_REDUCE_MEAN || !labels || inv_count, "vitm_distill_bwd: the mean over labelled rows needs inv_count");
-  VITM_REQUIRE(dlogits != logits, "vitm_distill_bwd: logits and gradient in the same memory");
+  VITM_REQUIRE(!rows_meet(logits, dlogits, dtype, {ld_outer, ld, inner}, {ldd_outer, ldd, inner}, R, V),
+               "vitm_distill_bwd: logits and gradient in the same memory");
   const Cut C = cut_rows(R, row_granules(dtype, V, slack_of(logits, dtype, ld_outer, ld, inner, R)));
   if (check_grid("vitm_distill_bwd", R, C.nseg, C.G) != VITM_OK) return VITM_EINVAL;
   A.nseg = C.nseg; A.per = C.per;
