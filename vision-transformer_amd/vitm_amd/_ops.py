@@ -65,6 +65,21 @@ def _dt(t: torch.Tensor) -> int:
     raise TypeError(f"unsupported dtype {t.dtype} (bf16 or fp32)")
 
 
+_held = None
+
+
+@contextlib.contextmanager
+def holding(kept: list):
+    """What is handed to kernels as weights in here (packed ones and fp32 vectors) joins ``kept``.  A captured graph keeps the
+    addresses of such memory only: held by its owner, it stays when the module packs new weights."""
+    global _held
+    before, _held = _held, kept
+    try:
+        yield
+    finally:
+        _held = before
+
+
 def f32vec(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """A parameter vector as a contiguous fp32 tensor: no copy when it already is one, otherwise a copy that is
     memoised on the tensor until its storage or version changes (so a bf16 module converts once, not per call)."""
@@ -72,16 +87,20 @@ def f32vec(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
         return None
     d = t.detach()
     if d.dtype == torch.float32 and d.is_contiguous():
-        return d
-    key = (t.data_ptr(), t._version, t.dtype, t.device, tuple(t.shape))
-    hit = getattr(t, "_vitm_f32", None)
-    if hit is not None and hit[0] == key:
-        return hit[1]
-    val = d.to(torch.float32).contiguous()
-    try:
-        t._vitm_f32 = (key, val)
-    except AttributeError:  # pragma: no cover - tensors that refuse attributes just convert every time
-        pass
+        val = d
+    else:
+        key = (t.data_ptr(), t._version, t.dtype, t.device, tuple(t.shape))
+        hit = getattr(t, "_vitm_f32", None)
+        if hit is not None and hit[0] == key:
+            val = hit[1]
+        else:
+            val = d.to(torch.float32).contiguous()
+            try:
+                t._vitm_f32 = (key, val)
+            except AttributeError:  # pragma: no cover - tensors that refuse attributes just convert every time
+                pass
+    if _held is not None:
+        _held.append(val)
     return val
 
 
@@ -139,9 +158,12 @@ def cached_pack(owner, slot: str, tensors: Sequence[Optional[torch.Tensor]], bui
     cache = owner.__dict__.setdefault("_vitm_packs", {})
     hit = cache.get(slot)
     if hit is not None and hit[0] == key:
-        return hit[1]
-    val = build()
-    cache[slot] = (key, val)
+        val = hit[1]
+    else:
+        val = build()
+        cache[slot] = (key, val)
+    if _held is not None:
+        _held.append(val)
     return val
 
 

@@ -11,6 +11,8 @@ from __future__ import annotations
 
 import torch
 
+from . import _ops
+
 
 class GraphedForward:
     """``g = GraphedForward(module, example_input)`` then ``y = g(x)`` for any ``x`` of that shape and dtype.
@@ -58,8 +60,10 @@ class GraphedTrainStep:
     launch, ``scheduler.step()``.  The kernels and their order are those of the eager step.  Needs the flat AdamW of this
     package, a single process (no gradient all-reduce) and batches of one shape; the returned loss is a copy.
 
-    A teacher of the trainer's is captured with the step, its weights as they are then: a module whose parameters change
-    afterwards is refused (hand ``step`` the ``teacher_top`` of such a teacher), any other callable has to stay what it was.
+    A teacher of the trainer's is captured with the step, its weights as they are then.  A module whose parameters were
+    written in place, moved, cast or replaced since is refused (hand ``step`` the ``teacher_top`` of such a teacher), and so
+    are another teacher and other settings of the distillation loss.  A write through ``p.data`` leaves no trace that could
+    be looked at and goes unseen; a teacher that is no module has to stay what it was.
     """
 
     def __init__(self, trainer, warmup: int = 2):
@@ -68,21 +72,36 @@ class GraphedTrainStep:
         self.trainer, self.warmup, self.calls = trainer, max(1, int(warmup)), 0
         self.graph = None
 
-    def _teacher_versions(self):
-        """What the captured teacher's packed weights were made from (none where no teacher module is in the graph)."""
-        t = self.trainer.teacher
-        return [p._version for p in t.parameters()] if self.top is None and isinstance(t, torch.nn.Module) else None
+    def _distilled_from(self):
+        """(settings of the loss, what the captured teacher's weights were made from): the latter is what packed weights are
+        kept by; buffers are read where they are, so only their place counts."""
+        tr = self.trainer
+        if tr.distillation is None:
+            return None, None
+        t = tr.teacher
+        if self.top is not None:
+            weights = None
+        elif not isinstance(t, torch.nn.Module):
+            weights = t
+        else:
+            weights = (t, [(p.data_ptr(), p._version, p.dtype, p.device) for p in t.parameters()],
+                       [(b.data_ptr(), b.dtype, b.device) for b in t.buffers()])
+        return tr.distillation._cfg(), (tr.teacher_top_k if self.top is None else None, weights)
 
     def _capture(self, images, labels, teacher_top):
         tr = self.trainer
         dev = images.device
         self.x, self.y = images.detach().clone(), labels.detach().clone()
         self.top = None if teacher_top is None else tuple(t.detach().clone() for t in teacher_top)
-        self.teacher_versions = self._teacher_versions()
+        self.distilled_from = self._distilled_from()
+        # what the graph's kernels read has to outlive whatever becomes of the teacher
+        self.held = []
+        if self.top is None and isinstance(tr.teacher, torch.nn.Module):
+            self.held += [t.detach() for t in (*tr.teacher.parameters(), *tr.teacher.buffers())]
         self.hyper = torch.zeros(8, dtype=torch.float32, device=dev)
         torch.cuda.synchronize(dev)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        with _ops.holding(self.held), torch.cuda.graph(self.graph):
             self.loss, self.norm = tr.device_step(self.x, self.y, self.hyper, self.top)
 
     def step(self, images: torch.Tensor, labels: torch.Tensor, teacher_top=None) -> torch.Tensor:
@@ -99,8 +118,12 @@ class GraphedTrainStep:
         for mine, t in zip(self.top or (), teacher_top or ()):
             if t.shape != mine.shape or t.dtype != mine.dtype:
                 raise RuntimeError(f"captured for teacher_top {tuple(mine.shape)} {mine.dtype}, got {tuple(t.shape)} {t.dtype}")
-        if self._teacher_versions() != self.teacher_versions:
-            raise RuntimeError("the teacher's weights changed after the step was captured: capture anew, or a step that is given teacher_top")
+        settings, teacher = self._distilled_from()
+        if settings != self.distilled_from[0]:
+            raise RuntimeError("the settings of the distillation loss changed after the step was captured: capture anew")
+        if teacher != self.distilled_from[1]:
+            raise RuntimeError("the teacher, or the teacher's weights, changed after the step was captured: capture anew, or a step "
+                               "that is given teacher_top")
         if not tr.optimizer._flat_ok():
             raise RuntimeError("the parameters or gradients left the flat buffers the graph was captured on")
         vals = tr.optimizer.next_hyper()
