@@ -477,6 +477,24 @@ def test_graph_replay_survives_other_batch_shapes():
     assert torch.equal(before, eager) and torch.equal(after, eager)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_graph_replay_survives_new_weights(dtype):
+    """A captured forward owns the weights it reads: after the module got others and packed them, the replay is still the old
+    result bit for bit."""
+    from vitm_amd import GraphedForward
+    model, sd, cfg = build("vit_tiny_cifar", seed=2)
+    x = torch.from_numpy(W.make_input(cfg, 16, 3)).cuda().to(dtype)
+    with torch.no_grad():
+        g = GraphedForward(model, x)
+        before = g(x).clone()
+        model.load_state_dict({k: v * 2 for k, v in model.state_dict().items()}, assign=True)
+        assert not torch.equal(model(x), before)
+        scribble = [torch.full((n,), float("nan"), device="cuda") for n in (1 << 24, 1 << 20, 1 << 16, 1 << 12, 768) for _ in range(8)]
+        after = g(x).clone()
+        del scribble
+    assert torch.equal(before, after)
+
+
 @pytest.mark.parametrize("name,batch", [("vit_tiny_cifar", 16), ("vit_s16", 4)])
 def test_graph_replay_is_bit_identical(name, batch):
     """The forward captured into a HIP graph replays the same kernels on the same buffers."""

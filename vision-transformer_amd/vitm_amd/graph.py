@@ -18,8 +18,8 @@ class GraphedForward:
     """``g = GraphedForward(module, example_input)`` then ``y = g(x)`` for any ``x`` of that shape and dtype.
 
     The returned tensor is the graph's static output buffer: it is overwritten by the next call (clone it to
-    keep it).  Weights are read from the module's packed copies as they were at capture time; re-capture after
-    changing them.
+    keep it).  Weights are read from the module's packed copies as they were at capture time (the graph
+    keeps that memory, whatever becomes of the module); re-capture after changing them.
     """
 
     def __init__(self, module: torch.nn.Module, example: torch.Tensor, warmup: int = 2):
@@ -35,8 +35,8 @@ class GraphedForward:
                     module(self.static_in)
             torch.cuda.current_stream(example.device).wait_stream(side)
             torch.cuda.synchronize(example.device)
-            self.graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph):
+            self.graph, self.held = torch.cuda.CUDAGraph(), []
+            with _ops.holding(self.held), torch.cuda.graph(self.graph):
                 self.static_out = module(self.static_in)
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
