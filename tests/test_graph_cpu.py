@@ -138,3 +138,13 @@ def test_captured_step_keeps_what_its_kernels_read(graphed):
     del g, step
     tr.device_step = None
     assert made[0]() is None
+
+
+def test_captured_step_takes_both_parts_of_teacher_top(graphed):
+    """A tuple of another length would leave the captured indices as they were."""
+    top = (torch.zeros(2, 4), torch.zeros(2, 4, dtype=torch.int64))
+    g, tr, _ = graphed(None, top=top)
+    for bad in ((torch.ones(2, 4),), (*top, torch.ones(2, 4))):
+        with pytest.raises(RuntimeError, match="log probabilities, indices"):
+            g.step(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64), bad)
+    assert tr.optimizer.steps == 2

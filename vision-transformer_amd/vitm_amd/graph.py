@@ -115,6 +115,8 @@ class GraphedTrainStep:
             raise RuntimeError(f"captured for images {tuple(self.x.shape)} {self.x.dtype}, got {tuple(images.shape)} {images.dtype}")
         if (teacher_top is None) != (self.top is None):
             raise RuntimeError("captured with teacher_top, got none" if teacher_top is None else "captured without teacher_top")
+        if len(teacher_top or ()) != len(self.top or ()):
+            raise RuntimeError(f"teacher_top is (log probabilities, indices), got {len(teacher_top)} entries")
         for mine, t in zip(self.top or (), teacher_top or ()):
             if t.shape != mine.shape or t.dtype != mine.dtype:
                 raise RuntimeError(f"captured for teacher_top {tuple(mine.shape)} {mine.dtype}, got {tuple(t.shape)} {t.dtype}")
