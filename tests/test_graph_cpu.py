@@ -148,3 +148,25 @@ def test_captured_step_takes_both_parts_of_teacher_top(graphed):
         with pytest.raises(RuntimeError, match="log probabilities, indices"):
             g.step(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64), bad)
     assert tr.optimizer.steps == 2
+
+
+def test_a_capture_that_failed_is_not_replayed(graphed):
+    from vitm_amd import GraphedTrainStep
+    _, tr, _ = graphed(None, top=(torch.zeros(2, 4), torch.zeros(2, 4, dtype=torch.int64)))
+    good, fails = tr.device_step, []
+
+    def device_step(*a):
+        if not fails:
+            fails.append(1)
+            raise ValueError("refused")
+        return good(*a)
+
+    tr.device_step = device_step
+    g = GraphedTrainStep(tr, warmup=1)
+    args = (torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64), (torch.zeros(2, 4), torch.zeros(2, 4, dtype=torch.int64)))
+    g.step(*args)
+    with pytest.raises(ValueError, match="refused"):
+        g.step(*args)
+    assert g.graph is None and tr.optimizer.steps == 2
+    g.step(*args)
+    assert g.graph is not None and tr.optimizer.steps == 3

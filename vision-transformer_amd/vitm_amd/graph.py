@@ -100,9 +100,10 @@ class GraphedTrainStep:
             self.held += [t.detach() for t in (*tr.teacher.parameters(), *tr.teacher.buffers())]
         self.hyper = torch.zeros(8, dtype=torch.float32, device=dev)
         torch.cuda.synchronize(dev)
-        self.graph = torch.cuda.CUDAGraph()
-        with _ops.holding(self.held), torch.cuda.graph(self.graph):
+        graph = torch.cuda.CUDAGraph()
+        with _ops.holding(self.held), torch.cuda.graph(graph):
             self.loss, self.norm = tr.device_step(self.x, self.y, self.hyper, self.top)
+        self.graph = graph
 
     def step(self, images: torch.Tensor, labels: torch.Tensor, teacher_top=None) -> torch.Tensor:
         tr = self.trainer
