@@ -273,3 +273,15 @@ def test_c_abi_refuses_a_gradient_that_meets_the_logits():
     all_refuse(at(0), 0, 0, R, at(4), 0, 9)            # one row of logits, repeated
     all_refuse(at(0), 100, 10, 3, at(35), 60, 11)      # two strides
     all_refuse(at(85), 9, 1, 3, at(0), 60, 11)
+
+
+def test_more_rows_than_the_c_abi_counts_are_refused(log_probs, DistillationLoss):
+    """2^32 + 5 rows would arrive as 5."""
+    z = torch.zeros(1, 2).expand(2 ** 32 + 5, 2)
+    with pytest.raises(ValueError, match="4294967301 rows"):
+        log_probs(z)
+    each = lambda t: t.expand(2 ** 32 + 5, 1)
+    with pytest.raises(ValueError, match="4294967301 rows"):
+        DistillationLoss()(z, each(torch.zeros(1, 1)), each(torch.zeros(1, 1, dtype=torch.int64)))
+    with pytest.raises(RuntimeError, match="MI355X"):
+        log_probs(torch.zeros(1, 2).expand(2 ** 30, 2))

@@ -29,6 +29,8 @@ def check_scores(logits: torch.Tensor, temperature: float, what: str) -> None:
         raise TypeError(f"{what}: unsupported logits dtype {logits.dtype} (bf16 or fp32)")
     if not 1 <= logits.shape[-1] <= _lib.SCORES_MAX_CLASSES:
         raise ValueError(f"{what}: {logits.shape[-1]} classes, supported are 1 to {_lib.SCORES_MAX_CLASSES}")
+    if logits.numel() > _lib.SCORES_MAX_ROWS * logits.shape[-1]:
+        raise ValueError(f"{what}: {logits.numel() // logits.shape[-1]} rows, supported are at most {_lib.SCORES_MAX_ROWS}")
     check_temperature(temperature, what)
 
 
