@@ -709,3 +709,22 @@ def test_gradient_interleaved_with_the_logits(dtype):
                                 torch.cuda.current_stream().cuda_stream), "distill")
     assert torch.equal(z, kept)
     _check_distill(z, tl, idx, None, row_loss, out, 1.0, 0.0, True)
+
+
+def test_very_many_short_rows(log_probs, Loss):
+    """More rows than 1024 threads each would leave room for."""
+    R, V = (1 << 22) + 3, 10
+    z = torch.randn(R, V, generator=torch.Generator(DEV).manual_seed(1), device=DEV)
+    idx = torch.arange(3, device=DEV).expand(R, 3)
+    tl = torch.log_softmax(z[:, :4] * 0.5, 1)[:, :3].contiguous()
+    labels = torch.arange(R, device=DEV) % V
+    labels[::7] = -100
+    loss, dz = Loss(2.0, 0.5, True, "none").loss_and_grad(z, tl, idx, labels)
+    for a in (0, R // 2, R - 1000):               # (the oracle takes 64 bits a class)
+        part = slice(a, a + 1000)
+        _check_distill(z[part], tl[part], idx[part], labels[part], loss[part], dz[part], 2.0, 0.5, True)
+    n = int((labels != -100).sum())
+    mean, dm = Loss(2.0, 0.5, True).loss_and_grad(z, tl, idx, labels)
+    # a thread adds 4097 rows, then 6 + 15 across the workgroup; each row's loss counts as it is
+    _near(mean, loss.double().sum() / n, U * 4200 * loss.double().abs().sum() / n, "mean")
+    assert (dm - dz / n).abs().max() <= 4 * U * dz.abs().max() / n

@@ -285,3 +285,23 @@ def test_more_rows_than_the_c_abi_counts_are_refused(log_probs, DistillationLoss
         DistillationLoss()(z, each(torch.zeros(1, 1)), each(torch.zeros(1, 1, dtype=torch.int64)))
     with pytest.raises(RuntimeError, match="MI355X"):
         log_probs(torch.zeros(1, 2).expand(2 ** 30, 2))
+
+
+def test_rows_beyond_one_launch_are_refused_by_what_is_launched():
+    """fewer than 2^32 threads: 2^22 rows of 1024 threads are too many, 2^22 rows of 64 are not (test_gpu_scores.py runs more)."""
+    from vitm_amd import _lib
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(4096)
+    p = ctypes.c_void_p((ctypes.addressof(buf) + 255) & ~255)
+    f = ctypes.c_float
+
+    def refused(rc):
+        assert rc == -1 and b"exceed one launch" in lib.vitm_last_error(), (rc, lib.vitm_last_error())
+
+    R, V = 1 << 22, 300000                        # a row of more than 32768 granules; every row the same one
+    refused(lib.vitm_log_probs(p, _lib.BF16, 0, 0, R, R, V, f(1.0), p, 1, -100, 2, p, p, p, p, p, p, None))
+    R = 1 << 24                                   # 256 threads a row
+    refused(lib.vitm_log_probs(p, _lib.BF16, 0, 0, R, R, 5000, f(1.0), p, 1, -100, 2, p, p, p, p, p, p, None))
+    refused(lib.vitm_distill(p, _lib.BF16, 0, 0, R, R, 5000, f(1.0), f(0.0), 0, p, p, 4, None, -100, 2, p, p, p, p, None, 0, 0, None))
+    R = 1 << 26                                   # 64
+    refused(lib.vitm_log_probs(p, _lib.BF16, 0, 0, R, R, 8, f(1.0), p, 1, -100, 2, p, p, p, p, p, p, None))

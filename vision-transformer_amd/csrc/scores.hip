@@ -1392,8 +1392,8 @@ int check_temperature(const char* what, float t) {
   return VITM_OK;
 }
 // a grid holds fewer than 2^32 threads
-int check_grid(const char* what, int R, int nseg, int threads) {
-  VITM_REQUIRE((int64_t)R * nseg * threads < (1ll << 32), "%s: %d rows exceed one launch", what, R);
+int check_grid(const char* what, int R, int64_t workgroups, int threads) {
+  VITM_REQUIRE(workgroups * threads < (1ll << 32), "%s: %d rows exceed one launch", what, R);
   return VITM_OK;
 }
 
@@ -1408,10 +1408,13 @@ int check_grid(const char* what, int R, int nseg, int threads) {
     else { CALL(1024, 4); }                                                                                             \
   } while (0)
 
-template <typename T> int launch_log_probs(const LogProbsArgs& A, int nq, hipStream_t st) {
-  Plan P = plan_rows(A.R, nq);
+Plan plan_log_probs(int R, int nq, int top_k) {
+  if (top_k == 0 && nq <= 16) return {nq <= 4 ? 4 : 16, 1};
+  const Plan P = plan_rows(R, nq);
+  return top_k > 0 && P.G == 256 && nq > kTopChunks * 1024 ? Plan{1024, 4} : P;   // the cells of a row fit LDS
+}
+template <typename T> int launch_log_probs(const LogProbsArgs& A, const Plan& P, int nq, hipStream_t st) {
   if (A.K == 0) {
-    if (nq <= 16) P = {nq <= 4 ? 4 : 16, 1};
 #define LP(G, NV) SCORES_LAUNCH((log_probs_kernel<T, G, NV>), cover(A.R, rows_of_group(G)), G * rows_of_group(G), 0, A)
     if (P.G == 4) LP(4, 1);
     else if (P.G == 16) LP(16, 1);
@@ -1421,7 +1424,7 @@ template <typename T> int launch_log_probs(const LogProbsArgs& A, int nq, hipStr
     if (P.NV == 1) SCORES_LAUNCH((log_probs_wave_top_kernel<T, 1>), A.R, 64, 0, A);
     else if (P.NV == 2) SCORES_LAUNCH((log_probs_wave_top_kernel<T, 2>), A.R, 64, 0, A);
     else SCORES_LAUNCH((log_probs_wave_top_kernel<T, 4>), A.R, 64, 0, A);
-  } else if (P.G == 256 && nq <= kTopChunks * 1024) {
+  } else if (P.G == 256) {
     SCORES_LAUNCH((log_probs_top_kernel<T, 256, 4>), A.R, 256, cover(nq, 1024) * 1024, A);
   } else {
     VITM_LDS_OPTIN((log_probs_top_kernel<T, 1024, 4>), kTopChunks * 4096, "vitm_log_probs");
@@ -1438,8 +1441,7 @@ template <typename T> void launch_log_probs_bwd(const LogProbsBwdArgs& A, const 
 #undef LPB
 }
 constexpr int kMarks = 131072;   // most granules of a row: the marks of the tail form
-template <typename T, bool GRAD> int launch_distill_rows(const DistillArgs& A, int nq, hipStream_t st) {
-  const Plan P = plan_rows(A.R, nq);
+template <typename T, bool GRAD> int launch_distill_rows(const DistillArgs& A, const Plan& P, int nq, hipStream_t st) {
   const int lds = A.tail ? cover(nq, 4) * 4 : 0;
 #define DS(G, NV)                                                                                                       \
   if (lds > 32768) VITM_LDS_OPTIN((distill_rows_kernel<T, G, NV, GRAD>), kMarks, "vitm_distill");                       \
@@ -1457,17 +1459,25 @@ template <typename T, bool GRAD> int launch_distill_rows(const DistillArgs& A, i
 // no classes have to be taken out of the sums (4096 x 32000 bf16: 117 us against 135 us with a second reading; 2048 x 32000 fp32:
 // 106 against 131); with the tail's marks the walk is the faster one (4096 x 50001 bf16: 211 us against 253 us held).  A row of
 // 16384 granules fills the registers of a CU, and nothing runs beside its phases: 640 us against 500 us at 4096 x 131072 bf16.
-template <typename T> int launch_distill_fused(const DistillArgs& A, int nq, hipStream_t st) {
+Plan plan_distill_fused(int R, int nq, bool tail) {   // NV = 0: a walk by launch_distill_rows
+  if (nq <= 1024 || (!tail && nq <= 8192)) {
+    if (nq <= 256) return {64, nq <= 64 ? 1 : nq <= 128 ? 2 : 4};
+    if (nq <= 4096) return {256, nq <= 1024 ? 4 : nq <= 2048 ? 8 : 16};
+    return {512, 16};
+  }
+  return {plan_rows(R, nq).G, 0};
+}
+template <typename T> int launch_distill_fused(const DistillArgs& A, const Plan& P, int nq, hipStream_t st) {
+  if (P.NV == 0) return launch_distill_rows<T, true>(A, P, nq, st);
   const int lds = A.tail ? cover(nq, 4) * 4 : 0;
 #define DH(G, NV) SCORES_LAUNCH((distill_held_kernel<T, G, NV>), A.R, G, lds, A)
-  if (nq <= 64) DH(64, 1);
-  else if (nq <= 128) DH(64, 2);
-  else if (nq <= 256) DH(64, 4);
-  else if (nq <= 1024) DH(256, 4);
-  else if (A.tail || nq > 8192) return launch_distill_rows<T, true>(A, nq, st);
-  else if (nq <= 2048) DH(256, 8);
-  else if (nq <= 4096) DH(256, 16);
-  else DH(512, 16);
+  if (P.G == 64 && P.NV == 1) DH(64, 1);
+  else if (P.G == 64 && P.NV == 2) DH(64, 2);
+  else if (P.G == 64) DH(64, 4);
+  else if (P.G == 512) DH(512, 16);
+  else if (P.NV == 4) DH(256, 4);
+  else if (P.NV == 8) DH(256, 8);
+  else DH(256, 16);
 #undef DH
   return VITM_OK;
 }
@@ -1505,9 +1515,11 @@ extern "C" int vitm_log_probs(const void* logits, int dtype, int64_t ld_outer, i
   A.targets = targets; A.G = n_targets; A.ignore = ignore_index; A.K = top_k;
   A.logprobs = logprobs; A.lse = lse; A.entropy = entropy; A.top_lp = top_logprobs; A.top_idx = top_indices; A.stats = stats;
   const int nq = row_granules(dtype, V, slack_of(logits, dtype, ld_outer, ld, inner, R));
-  if (check_grid("vitm_log_probs", R, 1, plan_rows(R, nq).G) != VITM_OK) return VITM_EINVAL;
+  const Plan P = plan_log_probs(R, nq, top_k);
+  // short rows, several to a wave, are held to the number that a wave each would allow
+  if (check_grid("vitm_log_probs", R, R, P.G < 64 ? 64 : P.G) != VITM_OK) return VITM_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  const int rl = dtype == VITM_BF16 ? launch_log_probs<bf16_t>(A, nq, st) : launch_log_probs<float>(A, nq, st);
+  const int rl = dtype == VITM_BF16 ? launch_log_probs<bf16_t>(A, P, nq, st) : launch_log_probs<float>(A, P, nq, st);
   if (rl != VITM_OK) return rl;
   VITM_CHECK_LAUNCH("vitm_log_probs");
   return VITM_OK;
@@ -1531,7 +1543,7 @@ extern "C" int vitm_log_probs_bwd(const void* logits, int dtype, int64_t ld_oute
   VITM_REQUIRE(!rows_meet(logits, dlogits, dtype, {ld_outer, ld, inner}, {ldd_outer, ldd, inner}, R, V),
                "vitm_log_probs_bwd: logits and gradient in the same memory");
   const Cut C = cut_rows(R, row_granules(dtype, V, slack_of(logits, dtype, ld_outer, ld, inner, R)));
-  if (check_grid("vitm_log_probs_bwd", R, C.nseg, C.G) != VITM_OK) return VITM_EINVAL;
+  if (check_grid("vitm_log_probs_bwd", R, (int64_t)R * C.nseg, C.G) != VITM_OK) return VITM_EINVAL;
   LogProbsBwdArgs A = {};
   A.logits = logits;
   A.at = {ld_outer, ld, inner};
@@ -1593,7 +1605,8 @@ extern "C" int vitm_distill(const void* logits, int dtype, int64_t ld_outer, int
                  "vitm_distill: logits and gradient in the same memory");
   }
   const int nq = row_granules(dtype, V, slack_of(logits, dtype, ld_outer, ld, inner, R));
-  if (check_grid("vitm_distill", R, 1, 1024) != VITM_OK) return VITM_EINVAL;
+  const Plan P = dlogits ? plan_distill_fused(R, nq, tail != 0) : plan_rows(R, nq);
+  if (check_grid("vitm_distill", R, R, P.G) != VITM_OK) return VITM_EINVAL;
   A.row_loss = row_loss;
   A.state = state;
   A.dlogits = dlogits;
@@ -1611,8 +1624,8 @@ extern "C" int vitm_distill(const void* logits, int dtype, int64_t ld_outer, int
       }
     }
   }
-  const int rl = dlogits ? (bf ? launch_distill_fused<bf16_t>(A, nq, st) : launch_distill_fused<float>(A, nq, st))
-                         : (bf ? launch_distill_rows<bf16_t, false>(A, nq, st) : launch_distill_rows<float, false>(A, nq, st));
+  const int rl = dlogits ? (bf ? launch_distill_fused<bf16_t>(A, P, nq, st) : launch_distill_fused<float>(A, P, nq, st))
+                         : (bf ? launch_distill_rows<bf16_t, false>(A, P, nq, st) : launch_distill_rows<float, false>(A, P, nq, st));
   if (rl != VITM_OK) return rl;
   if (reduction != VITM_REDUCE_NONE)
     hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, st, (const float*)row_loss,
@@ -1636,7 +1649,7 @@ extern "C" int vitm_distill_bwd(const void* logits, int dtype, int64_t ld_outer,
   VITM_REQUIRE(!rows_meet(logits, dlogits, dtype, {ld_outer, ld, inner}, {ldd_outer, ldd, inner}, R, V),
                "vitm_distill_bwd: logits and gradient in the same memory");
   const Cut C = cut_rows(R, row_granules(dtype, V, slack_of(logits, dtype, ld_outer, ld, inner, R)));
-  if (check_grid("vitm_distill_bwd", R, C.nseg, C.G) != VITM_OK) return VITM_EINVAL;
+  if (check_grid("vitm_distill_bwd", R, (int64_t)R * C.nseg, C.G) != VITM_OK) return VITM_EINVAL;
   A.nseg = C.nseg; A.per = C.per;
   A.state = (float*)state;
   A.upstream = upstream;
