@@ -305,3 +305,20 @@ def test_rows_beyond_one_launch_are_refused_by_what_is_launched():
     refused(lib.vitm_distill(p, _lib.BF16, 0, 0, R, R, 5000, f(1.0), f(0.0), 0, p, p, 4, None, -100, 2, p, p, p, p, None, 0, 0, None))
     R = 1 << 26                                   # 64
     refused(lib.vitm_log_probs(p, _lib.BF16, 0, 0, R, R, 8, f(1.0), p, 1, -100, 2, p, p, p, p, p, p, None))
+
+
+def test_forward_mode_is_refused(log_probs, DistillationLoss):
+    """A dual tensor asks for no gradient, so its tangent would be left out in silence."""
+    from torch.autograd import forward_ad as fw
+    z, tl, idx = torch.zeros(3, 9), torch.zeros(3, 4), torch.zeros(3, 4, dtype=torch.int64)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))
+        for f in (lambda: log_probs(dual(z)), lambda: log_probs(dual(z[:0])), lambda: DistillationLoss()(dual(z), tl, idx),
+                  lambda: DistillationLoss().loss_and_grad(dual(z), tl, idx), lambda: DistillationLoss()(z, dual(tl), idx),
+                  lambda: DistillationLoss().loss_and_grad(z, dual(tl), idx)):
+            with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                f()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                f()
+        with pytest.raises(RuntimeError, match="MI355X"):
+            log_probs(z)                          # a plain tensor inside a dual level

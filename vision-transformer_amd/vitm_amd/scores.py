@@ -7,6 +7,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, _ops
 from . import _score_ops as S
@@ -32,6 +33,14 @@ def check_scores(logits: torch.Tensor, temperature: float, what: str) -> None:
     if logits.numel() > _lib.SCORES_MAX_ROWS * logits.shape[-1]:
         raise ValueError(f"{what}: {logits.numel() // logits.shape[-1]} rows, supported are at most {_lib.SCORES_MAX_ROWS}")
     check_temperature(temperature, what)
+    refuse_tangents(what, logits)
+
+
+def refuse_tangents(what: str, *inputs: torch.Tensor) -> None:
+    """A dual tensor's values alone would pass for a derivative of 0."""
+    for t in inputs:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def check_temperature(temperature: float, what: str) -> None:

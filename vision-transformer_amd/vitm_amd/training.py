@@ -612,6 +612,7 @@ class DistillationLoss(nn.Module):
             raise TypeError(f"{what}: unsupported dtype {teacher.dtype} of the teacher's log probabilities (bf16 or fp32)")
         if teacher.device != logits.device:
             raise RuntimeError(f"{what}: the teacher's log probabilities are on {teacher.device}, the logits on {logits.device}")
+        scores.refuse_tangents(what, teacher)
         if tracked and teacher.requires_grad:
             raise ValueError(f"{what}: no gradient flows to the teacher; detach its log probabilities")
         scores.check_indices(indices, logits, f"{what}: indices")
