@@ -728,3 +728,16 @@ def test_very_many_short_rows(log_probs, Loss):
     # a thread adds 4097 rows, then 6 + 15 across the workgroup; each row's loss counts as it is
     _near(mean, loss.double().sum() / n, U * 4200 * loss.double().abs().sum() / n, "mean")
     assert (dm - dz / n).abs().max() <= 4 * U * dz.abs().max() / n
+
+
+@pytest.mark.parametrize("R", [2, 777, 1024, 1025, 4100])
+def test_the_mean_is_that_of_the_rows(Loss, R):
+    """The sum of the rows' losses is taken in 64 bits and divided once: off the losses' mean by its own rounding, half a step."""
+    z = _scores(R, 40, F32, R)
+    tl, idx = _teacher(R, 40, 6, 1)
+    for labels in (None, torch.where(torch.arange(R, device=DEV) % 5 == 1, -100, 3)):
+        for red, n in (("sum", 1), ("mean", R if labels is None else int((labels != -100).sum()))):
+            rows = Loss(2.0, 0.0, False, "none")(z, tl, idx, labels).double()
+            exact = rows.sum() / n
+            got = Loss(2.0, 0.0, False, red)(z, tl, idx, labels)
+            assert (got.double() - exact).abs() <= exact.abs() * U * 1.0001, (red, labels is None)

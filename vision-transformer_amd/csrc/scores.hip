@@ -222,8 +222,19 @@ template <int CTRL> __device__ __forceinline__ float dpp(float v) {
 __device__ __forceinline__ float lane_value(float v, int lane) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
+struct Halves {
+  float lo, hi;
+};
+template <int CTRL> __device__ __forceinline__ double dpp(double v) {
+  const Halves h = __builtin_bit_cast(Halves, v);
+  return __builtin_bit_cast(double, Halves{dpp<CTRL>(h.lo), dpp<CTRL>(h.hi)});
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const Halves h = __builtin_bit_cast(Halves, v);
+  return __builtin_bit_cast(double, Halves{lane_value(h.lo, lane), lane_value(h.hi, lane)});
+}
 // op over groups of N neighbouring lanes, the same result in all of them
-template <int N, class Op> __device__ __forceinline__ float lane_reduce(float v, Op op) {
+template <int N, class F, class Op> __device__ __forceinline__ F lane_reduce(F v, Op op) {
   static_assert(N == 4 || N == 8 || N == 16 || N == 64, "groups of a quad, half a row, a row or the wave");
   v = op(v, dpp<0xB1>(v));                      // quad_perm 1 0 3 2
   v = op(v, dpp<0x4E>(v));                      // quad_perm 2 3 0 1
@@ -236,10 +247,10 @@ struct Max {
   __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
 };
 struct Add {
-  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+  template <class F> __device__ __forceinline__ F operator()(F a, F b) const { return a + b; }
 };
 __device__ __forceinline__ float wave_max(float v) { return lane_reduce<64>(v, Max()); }
-__device__ __forceinline__ float wave_add(float v) { return lane_reduce<64>(v, Add()); }
+template <class F> __device__ __forceinline__ F wave_add(F v) { return lane_reduce<64>(v, Add()); }
 template <int G> __device__ __forceinline__ float block_max(float v, float* sh) {
   v = wave_max(v);
   if constexpr (G > 64) {
@@ -1289,12 +1300,12 @@ __global__ __launch_bounds__(1024) void distill_count_kernel(const int64_t* labe
   const int c = count_rows<1024>(labels, ignore, R, cnt);
   if (threadIdx.x == 0) inv[0] = 1.f / (float)max(c, 1);
 }
-// the sum of the row losses times the scale; with labels the scale is 1 / counted rows, which is left in inv_count
+// the sum of the row losses over a count; with labels that of the counted rows, whose reciprocal is left in inv_count
 __global__ __launch_bounds__(1024) void distill_total_kernel(const float* rows, const int64_t* labels, int64_t ignore, int R,
-                                                             float host_scale, float* inv_count, float* loss) {
-  __shared__ float sh[16];
+                                                             float host_count, float* inv_count, float* loss) {
+  __shared__ double sh[16];
   __shared__ int cnt[16];
-  float s = 0.f;
+  double s = 0.;
   for (int i = threadIdx.x; i < R; i += 1024) s += rows[i];
   s = wave_add(s);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
@@ -1302,8 +1313,8 @@ __global__ __launch_bounds__(1024) void distill_total_kernel(const float* rows, 
   const int c = labels ? count_rows<1024>(labels, ignore, R, cnt) : 0;
   if (threadIdx.x == 0) {
     for (int w = 1; w < 16; ++w) s += sh[w];
-    if (labels) host_scale = inv_count[0] = 1.f / (float)max(c, 1);
-    loss[0] = s * host_scale;
+    if (labels) inv_count[0] = 1.f / (host_count = (float)max(c, 1));
+    loss[0] = (float)(s / host_count);
   }
 }
 
@@ -1629,7 +1640,8 @@ extern "C" int vitm_distill(const void* logits, int dtype, int64_t ld_outer, int
   if (rl != VITM_OK) return rl;
   if (reduction != VITM_REDUCE_NONE)
     hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, st, (const float*)row_loss,
-                       reduction == VITM_REDUCE_MEAN ? labels : nullptr, ignore_index, R, A.host_scale, inv_count, loss);
+                       reduction == VITM_REDUCE_MEAN ? labels : nullptr, ignore_index, R, reduction == VITM_REDUCE_MEAN ? (float)R : 1.f,
+                       inv_count, loss);
   VITM_CHECK_LAUNCH("vitm_distill");
   return VITM_OK;
 }
