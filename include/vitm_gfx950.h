@@ -409,7 +409,8 @@ int vitm_adamw_f32_hyper(float* p, const float* g, float* exp_avg, float* exp_av
 /* ---- class scores (logits): no counterpart in the reference -------------------------------------------------------
  * Rows of `V` scores in bf16 or fp32 (`dtype`), row r at element (r / inner) * ld_outer + (r % inner) * ld of `logits`
  * (a plain matrix: inner = R; a (batch, token, class) view: inner = tokens).  Rows need no alignment beyond their type's.
- * Class indices are int64.  Temperatures lie in [1e-6, 1e6].  At most vitm_scores_max_classes() classes, and lists (targets,
+ * Class indices are int64.  Temperatures lie in [1e-6, 1e6], those of
+ * distillation in [1e-6, 1e4].  At most vitm_scores_max_classes() classes, and lists (targets,
  * top classes, a teacher's list) of at most vitm_scores_max_top() entries a row.  At most as many rows as
  * one launch holds: fewer than 2^32 threads, of which a row counts 64 to 1024 by its length (more are refused).
  * A score of -inf is a masked class (probability 0).  A row with no other score has no distribution: its log

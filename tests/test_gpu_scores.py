@@ -741,3 +741,48 @@ def test_the_mean_is_that_of_the_rows(Loss, R):
             exact = rows.sum() / n
             got = Loss(2.0, 0.0, False, red)(z, tl, idx, labels)
             assert (got.double() - exact).abs() <= exact.abs() * U * 1.0001, (red, labels is None)
+
+
+@pytest.mark.parametrize("T", [4.0, 8.0, 9.0, 30.0, 1000.0, 10000.0])
+@pytest.mark.parametrize("R,V,K,tail,kind", [(64, 100, 100, False, ""), (64, 100, 100, True, ""), (64, 100, 20, True, ""), (64, 100, 99, False, ""),
+                                             (16, 5000, 64, True, ""), (16, 5000, 100, False, "masked"), (3, 40001, 100, True, ""),
+                                             (5, 40001, 128, False, "masked"), (16, 900, 30, True, "twice")])
+def test_distillation_at_high_temperatures(log_probs, Loss, R, V, K, tail, kind, T):
+    """The divergence shrinks with T^2 while its terms do not: the loss keeps its digits all the same.
+
+    With the listed classes apart (the tail form, or T above 8) all of the divergence's terms q d - q + p are positive and good to
+    some 30 u each.  The sums over the row are off by eps = 180 u at most (see above), which moves mass between list and rest:
+    eps |p_rest - q_rest| and eps^2 in the divergence; q_rest = 1 - sum q, of 7 + 1 additions and q good to 2 u, counts with
+    its d: 12 u |d_rest|.  Otherwise ln s is off by eps, and so is the divergence.  (A class listed twice has no small d.)"""
+    z, zt = _scores(R, V, F32, V, scale=2.0), _scores(R, V, F32, V + 1, scale=2.0)
+    if kind == "masked":                          # what the list leaves out is masked: its mass is 0 and has to come out so
+        z[:, K:] = NINF
+        zt[:, K:] = NINF
+    top = log_probs(zt, top_k=K, temperature=T)
+    tl, idx = top.top_logprobs, top.top_indices.clone()
+    if kind == "twice":
+        idx[:, 1] = idx[:, 0]
+    ref, mag, _, _ = O.distill(z, tl, idx, None, T, 0.0, tail)
+    p = torch.softmax(z.double() / T, 1)
+    listed = torch.zeros_like(p).scatter_(1, idx, 1.0) > 0
+    p_rest = torch.where(listed, torch.zeros_like(p), p).sum(1)
+    q_rest = (1 - tl.double().exp().sum(1)).clamp(min=0) if tail else torch.zeros_like(p_rest)
+    d = torch.where((q_rest > 0) & (p_rest > 0), (q_rest.log() - p_rest.log()).abs(), torch.zeros_like(p_rest))
+    eps = 180 * U
+    kl_tol = 30 * U * ref.abs() / T ** 2 + eps ** 2
+    if tail:
+        kl_tol = kl_tol + eps * (p_rest - q_rest).abs() + 12 * U * d
+    elif T > 8:
+        kl_tol = kl_tol + eps * p_rest
+    else:
+        kl_tol = kl_tol + eps
+    if kind == "twice":
+        kl_tol = kl_tol + 40 * U
+    loss, dz = Loss(T, 0.0, tail, "none").loss_and_grad(z, tl, idx)
+    _near(loss, ref, T ** 2 * kl_tol, "loss")
+    _check_distill(z, tl, idx, None, None, dz, T, 0.0, tail)
+    zr = z.clone().requires_grad_(True)
+    l2 = Loss(T, 0.0, tail, "none")(zr, tl, idx)
+    _near(l2.detach(), ref, T ** 2 * kl_tol, "loss")
+    (d2,) = torch.autograd.grad(l2, zr, torch.ones(R, device=DEV))
+    _check_distill(z, tl, idx, None, None, d2, T, 0.0, tail)

@@ -322,3 +322,20 @@ def test_forward_mode_is_refused(log_probs, DistillationLoss):
                 f()
         with pytest.raises(RuntimeError, match="MI355X"):
             log_probs(z)                          # a plain tensor inside a dual level
+
+
+def test_temperatures_of_distillation(DistillationLoss):
+    """Beyond 1e4 the gradient would have no digit left; log_probs has no such differences."""
+    with pytest.raises(ValueError, match="1e-6 to 10000"):
+        DistillationLoss(temperature=2e4)
+    loss = DistillationLoss(temperature=1e4)
+    loss.temperature = 2e4
+    with pytest.raises(ValueError, match="1e-6 to 10000"):
+        loss(**_args())
+    from vitm_amd import _lib
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(4096)
+    p, f = ctypes.c_void_p((ctypes.addressof(buf) + 255) & ~255), ctypes.c_float
+    rows = (p, 1, 0, 9, 3, 3, 9, f(2e4), f(0.0), 0, p, p, 4, None, -100, 2)
+    for rc in (lib.vitm_distill(*rows, p, p, p, p, None, 0, 0, None), lib.vitm_distill_bwd(*rows, p, p, p, p, 0, 9, None)):
+        assert rc == -1 and b"temperature" in lib.vitm_last_error()

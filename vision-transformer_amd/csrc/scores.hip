@@ -281,10 +281,12 @@ template <int G> __device__ __forceinline__ int block_total(int wave_uniform, in
 struct Sums {
   float m, s, s1, u;
 };
-// e^x, ln x and 1 / x by the hardware's base-2 functions: off by a unit or two of fp32 where they are used (arguments of ln are
-// 1 or more, or a mass of at least 2^-24)
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+// ln x by the hardware's base-2 function: off by a unit or two of fp32 where it is used (arguments of 1 or more)
 __device__ __forceinline__ float ln_of(float x) { return kLn2 * __builtin_amdgcn_logf(x); }
+// ln x to 4e-8 whatever its size: the exponent's part in 64 bits, the hardware's logarithm for the mantissa in [0.5, 1)
+__device__ __forceinline__ double wide_ln_of(float x) {
+  return fma((double)__builtin_amdgcn_frexp_expf(x), 0.6931471805599453, (double)ln_of(__builtin_amdgcn_frexp_mantf(x)));
+}
 __device__ __forceinline__ float rebase(float m, float M, float c) { return m == NINF ? 0.f : __builtin_amdgcn_exp2f((m - M) * c); }
 __device__ __forceinline__ void rebase_to(Sums& a, float M, float c, float c1) {
   const float w = rebase(a.m, M, c), t = a.m == NINF ? 0.f : (a.m - M) * c;
@@ -889,6 +891,7 @@ struct DistillArgs {
   int R, V, nseg, per;         // segments a row, granules a segment (gradient alone)
   float temperature, label_weight;
   int tail;
+  int apart;                   // the listed classes are taken out of the sums over the row (keeps_apart)
   const float* teacher;        // [R][K] log probabilities
   const int64_t* indices;      // [R][K], -1: absent
   int K;
@@ -906,12 +909,16 @@ struct DistillArgs {
 };
 struct __align__(16) ListScratch {
   int idx[kMaxTop];            // -1: absent
-  float q[kMaxTop], z[kMaxTop];   // the teacher's probabilities, the student's scores
-  float q_rest, Q, qlogq;      // tail mass of the teacher, mass of its list, sum of q ln q over the list
+  float l[kMaxTop], q[kMaxTop], z[kMaxTop];   // the teacher's log probabilities, its probabilities e^(l - norm), the student's scores
+  double norm;
+  float q_rest, Q;             // tail mass of the teacher, mass of its list
   int bad;                     // an index outside the classes
   int64_t y;                   // the label and its score
   float zy;
   RowState st;
+  Sums dn, tot;                // over the classes that the walk summed, and over all
+  bool others;                 // the walk saw classes
+  float fixed_loss;            // of a row without a gradient
   float scale;
 };
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
@@ -950,28 +957,26 @@ template <typename T> __device__ __forceinline__ void read_list(const DistillArg
     }
   }
   const float zy = y >= 0 && y < A.V ? Gran<T>::get(p + y) : 0.f;
-  float norm = 0.f;
+  double norm = 0.;
   if (!A.tail) {   // renormalised over the list
     float mx = wave_max(fmaxf(l[0], l[1]));
     mx = mx == NINF ? 0.f : mx;
-    norm = mx + ln_of(wave_add(exp_of(l[0] - mx) + exp_of(l[1] - mx)));
-    if (norm == NINF) norm = 0.f;   // nothing in the list
+    norm = mx + wide_ln_of(wave_add(expf(l[0] - mx) + (A.K > 64 ? expf(l[1] - mx) : 0.f)));
+    if (norm == NINF) norm = 0.;   // nothing in the list
   }
-  float ql = 0.f;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    q[h] = exp_of(l[h] - norm);
-    if (q[h] != 0.f) ql += q[h] * (l[h] - norm);
+    q[h] = A.K > 64 * h ? expf((float)(l[h] - norm)) : 0.f;
     L.idx[lane + 64 * h] = ix[h];
+    L.l[lane + 64 * h] = l[h];
     L.q[lane + 64 * h] = q[h];
     L.z[lane + 64 * h] = z[h];
   }
   const float Q = wave_add(q[0] + q[1]);
-  ql = wave_add(ql);
   const bool any_bad = __ballot(bad) != 0;
   if (lane == 0) {
     L.Q = Q;
-    L.qlogq = ql;
+    L.norm = norm;
     L.q_rest = A.tail ? fmaxf(1.f - Q, 0.f) : 0.f;
     L.bad = any_bad;
     L.y = y;
@@ -979,78 +984,127 @@ template <typename T> __device__ __forceinline__ void read_list(const DistillArg
   }
 }
 
-// wave 0: the loss of the row and its state from the sums over the row (in the tail form: over the classes outside the list)
-__device__ __forceinline__ void finish_row(const DistillArgs& A, int r, Sums dn, ListScratch& L) {
+// x - 1 + e^-x for |x| < 1: the series, without the cancellation around 0 (the first term left out is 2e-9)
+__device__ __forceinline__ float excess(float x) {
+  float p = -1.f / 39916800.f;
+  const float c[9] = {1.f / 3628800.f, -1.f / 362880.f, 1.f / 40320.f, -1.f / 5040.f, 1.f / 720.f, -1.f / 120.f, 1.f / 24.f, -1.f / 6.f, 0.5f};
+#pragma unroll
+  for (int i = 0; i < 9; ++i) p = fmaf(p, x, c[i]);
+  return p * x * x;
+}
+// wave 0: what the gradient of the row needs, from the sums over the row (`apart`: over the classes outside the list).  Returns
+// which of the lane's two entries are the first of their class.
+struct First {
+  bool at[2];
+};
+__device__ __forceinline__ First row_state(const DistillArgs& A, int r, Sums dn, ListScratch& L) {
   const int lane = threadIdx.x & 63;
-  const float T_ = A.temperature, inv_t = 1.f / T_, cT = inv_t * kLog2e, c1 = kLog2e, a = A.label_weight;
+  const float cT = kLog2e / A.temperature, c1 = kLog2e, a = A.label_weight;
   wave_sync();   // read_list's, where one wave has the row and met no barrier since
-  const float z[2] = {L.z[lane], L.z[lane + 64]}, q[2] = {L.q[lane], L.q[lane + 64]};
-  float q_rest = L.q_rest, Q = L.Q, tail_loss = 0.f;
-  if (dn.m == NINF && dn.s == 0.f) q_rest = 0.f;   // no class outside the list: no tail term
+  First first = {{false, false}};
   Sums tot = dn;
-  if (A.tail) {   // the listed classes join the sums, each once
-    bool first[2];
+  if (A.apart) {   // the listed classes join the sums, each once
+    const float z[2] = {L.z[lane], L.z[lane + 64]};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = lane + 64 * h, i = L.idx[k];
-      first[h] = i >= 0;
-      for_entries(L, A.K, i, [&](int j) { first[h] = first[h] && j >= k; });
+      first.at[h] = i >= 0;
+      for_entries(L, A.K, i, [&](int j) { first.at[h] = first.at[h] && j >= k; });
     }
     Sums o = {NINF, 0.f, 0.f, 0.f};
-    o.m = wave_max(fmaxf(first[0] ? z[0] : NINF, first[1] ? z[1] : NINF));
+    o.m = wave_max(fmaxf(first.at[0] ? z[0] : NINF, first.at[1] ? z[1] : NINF));
     const float b = o.m == NINF ? 0.f : o.m;
     float s = 0.f, s1 = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      if (first[h]) {
+      if (first.at[h]) {
         s += __builtin_amdgcn_exp2f((z[h] - b) * cT);
         s1 += __builtin_amdgcn_exp2f((z[h] - b) * c1);
       }
     o.s = wave_add(s);
     o.s1 = wave_add(s1);
     tot = merge<true, false>(dn, o, cT, c1);
-    if (q_rest > 0.f) {
-      // ln p_rest = ln(s_d 2^(cT (m_d - m))) - ln s
-      const float ln_rest = ln_of(dn.s) + (dn.m - tot.m) * inv_t - ln_of(tot.s);
-      tail_loss = q_rest * (ln_of(q_rest) - ln_rest);
-      Q += q_rest;
-    }
   }
-  const float ln_s = ln_of(tot.s), ln_s1 = ln_of(tot.s1);
-  float cross = 0.f;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    if (q[h] != 0.f) cross += q[h] * ((z[h] - tot.m) * inv_t - ln_s);
-  cross = wave_add(cross);
-  if (lane != 0) return;
+  if (lane != 0) return first;
+  const bool others = dn.m != NINF || dn.s != 0.f;     // classes outside the list (or NaN)
+  const float q_rest = others ? L.q_rest : 0.f, Q = L.Q + (A.apart ? q_rest : 0.f);   // none: no tail term
   const bool labelled = A.labels && L.y != A.ignore, skip = A.labels && L.y == A.ignore;
   const bool bad = L.bad || (labelled && (L.y < 0 || L.y >= A.V));
   const bool none = tot.m == NINF && tot.s == 0.f;
   RowState st = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  float loss = 0.f;
-  if (skip) {
-  } else if (bad) {
-    loss = __builtin_nanf("");
-  } else if (!none) {
-    const float kl = L.qlogq - cross + tail_loss;
-    loss = a == 1.f ? 0.f : (1.f - a) * T_ * T_ * kl;
-    if (a != 0.f) loss += a * (ln_s1 - (L.zy - tot.m));
-    st.cq = (1.f - a) * T_;
+  if (!skip && !bad && !none) {
+    st.cq = (1.f - a) * A.temperature;
     st.m = tot.m;
-    st.aT = st.cq * Q * __builtin_amdgcn_rcpf(tot.s);
-    st.a1 = a * __builtin_amdgcn_rcpf(tot.s1);
+    st.aT = st.cq * Q / tot.s;
+    st.a1 = a / tot.s1;
     st.md = dn.m == NINF ? 0.f : dn.m;
-    st.wT = st.aT * rebase(dn.m, tot.m, cT) - (q_rest > 0.f ? st.cq * q_rest * __builtin_amdgcn_rcpf(dn.s) : 0.f);
+    st.wT = st.aT * rebase(dn.m, tot.m, cT) - (q_rest > 0.f ? st.cq * q_rest / dn.s : 0.f);
     st.w1 = st.a1 * rebase(dn.m, tot.m, c1);
     st.ok = 1.f;
   }
-  A.row_loss[r] = loss;
   if (A.state) *(RowState*)(A.state + (int64_t)r * kState) = st;
   L.st = st;
+  L.dn = dn;
+  L.tot = tot;
+  L.others = others;
+  L.fixed_loss = !skip && bad ? __builtin_nanf("") : 0.f;
+  return first;
+}
+// wave 0: the loss of the row.  ln q - ln p of an entry is a difference of numbers that are larger than it by the temperature, and
+// the loss T^2 times a sum that is smaller by its square: logarithms and their differences are 64 bits.  Where the listed classes
+// are apart the sum is taken as that of q d - q + p over the list and the rest of the classes, d = ln q - ln p, which is the same
+// (the q and the p have one sum) and has no negative terms: what all p are off by together then hardly shows.
+__device__ __forceinline__ void row_loss(const DistillArgs& A, int r, const First& first, const ListScratch& L) {
+  const int lane = threadIdx.x & 63;
+  wave_sync();
+  if (L.st.ok == 0.f) {
+    if (lane == 0) A.row_loss[r] = L.fixed_loss;
+    return;
+  }
+  const float T_ = A.temperature, cT = kLog2e / T_, a = A.label_weight;
+  const double inv_t = 1. / (double)T_, norm = L.norm;
+  const Sums dn = L.dn, tot = L.tot;
+  const double ln_s = wide_ln_of(tot.s);
+  const float inv_s = 1.f / tot.s;
+  float kl = 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (64 * h >= A.K) break;
+    const float z = L.z[lane + 64 * h], q = L.q[lane + 64 * h];
+    const double x = ((double)z - (double)tot.m) * inv_t;
+    const float d = (float)((double)L.l[lane + 64 * h] - norm - x + ln_s);   // where q > 0
+    if (!A.apart) {
+      kl += q != 0.f ? q * d : 0.f;
+    } else {
+      const float p = first.at[h] ? __builtin_amdgcn_exp2f((z - tot.m) * cT) * inv_s : 0.f;
+      if (q == 0.f) kl += p;
+      else kl += first.at[h] && fabsf(d) < 1.f ? q * excess(d) : q * (d - 1.f) + p;
+    }
+  }
+  kl = wave_add(kl);
+  const float q_rest = L.others ? L.q_rest : 0.f;
+  double over = 0.;   // what the q are off a sum of 1, in the tail form without a tail
+  if (A.tail && q_rest == 0.f)
+    over = wave_add((L.idx[lane] >= 0 ? exp((double)L.l[lane]) : 0.) + (L.idx[lane + 64] >= 0 ? exp((double)L.l[lane + 64]) : 0.)) - 1.;
+  if (lane != 0) return;
+  if (A.apart) {
+    const float p = L.others ? dn.s * rebase(dn.m, tot.m, cT) * inv_s : 0.f;
+    if (q_rest > 0.f) {
+      const float d = (float)(wide_ln_of(q_rest) - wide_ln_of(dn.s) - ((double)dn.m - (double)tot.m) * inv_t + ln_s);
+      kl += fabsf(d) < 1.f ? q_rest * excess(d) : q_rest * (d - 1.f) + p;
+    } else if (A.tail) {
+      kl += p + (float)over;
+    } else {
+      kl = L.Q == 0.f ? 0.f : kl + p;    // 0: nothing listed
+    }
+  }
+  float loss = a == 1.f ? 0.f : (1.f - a) * T_ * T_ * kl;
+  if (a != 0.f) loss += a * (float)(wide_ln_of(tot.s1) - ((double)L.zy - (double)tot.m));
+  A.row_loss[r] = loss;
 }
 
-// tail form: one bit a class of the row (a byte a granule) says that the class is listed; such a class leaves the registers as
-// -inf, so that the sums run over the others
+// one bit a class of the row (a byte a granule) says that the class is listed; where the listed classes are apart such a class
+// leaves the registers as -inf, so that the sums run over the others
 template <typename T, int G>
 __device__ __forceinline__ void mark_listed(const Row<T>& row, int K, const ListScratch& L, unsigned* bits) {
   constexpr int E = Gran<T>::E;
@@ -1149,7 +1203,7 @@ __device__ __forceinline__ float scale_of(const DistillArgs& A, int r, int count
   return g;
 }
 
-// Rows of any length, in the tail form with the marks in dynamic LDS (one byte a granule).  With the gradient the row is read a
+// Rows of any length, where the listed classes are apart with the marks in dynamic LDS (one byte a granule).  With the gradient the row is read a
 // second time.
 template <typename T, int G, int NV, bool GRAD>
 __global__ __launch_bounds__(G) void distill_rows_kernel(DistillArgs A) {
@@ -1164,7 +1218,7 @@ __global__ __launch_bounds__(G) void distill_rows_kernel(DistillArgs A) {
   const bool two = A.temperature != 1.f && A.label_weight != 0.f;
   if (tid < 64) read_list<T>(A, row.p, r, L);
   Sums t;
-  if (A.tail) {
+  if (A.apart) {
     __syncthreads();
     mark_listed<T, G>(row, A.K, L, bits);
     const DropListed<T> drop = {(const unsigned char*)bits};
@@ -1175,12 +1229,14 @@ __global__ __launch_bounds__(G) void distill_rows_kernel(DistillArgs A) {
   if (!two) t.s1 = t.s;   // with one exponential both sums are the same numbers; for T != 1 without labels s1 is not used
   t = block_sums<G, true, false>(t, cT, two ? c1 : cT, sh);
   const int counted = GRAD && A.count_here ? count_rows<G>(A.labels, A.ignore, A.R, cnt) : 0;
-  if (tid < 64) finish_row(A, r, t, L);
+  First first;
+  if (tid < 64) first = row_state(A, r, t, L);
   if constexpr (GRAD) {
     if (tid == 0) L.scale = scale_of(A, r, counted);
     __syncthreads();
     grad_of_segment<T, G, NV>(A, row, r, 0, row.nq, L);
   }
+  if (tid < 64) row_loss(A, r, first, L);
 }
 
 // Loss and gradient of rows of up to G * NV granules, which stay in registers between the sums and the gradient: the row is read
@@ -1230,7 +1286,7 @@ __global__ __launch_bounds__(G) void distill_held_kernel(DistillArgs A) {
   u32x4_t edge = no_class<T>();
   if (eq >= 0) edge = load_edge(row, eq);
   if (tid < 64) read_list<T>(A, row.p, r, L);
-  if (A.tail) {
+  if (A.apart) {
     __syncthreads();
     mark_listed<T, G>(row, A.K, L, bits);
     const DropListed<T> drop = {(const unsigned char*)bits};
@@ -1243,12 +1299,14 @@ __global__ __launch_bounds__(G) void distill_held_kernel(DistillArgs A) {
   if (!two) t.s1 = t.s;
   t = block_sums<G, true, false>(t, cT, two ? c1 : cT, sh);
   const int counted = A.count_here ? count_rows<G>(A.labels, A.ignore, A.R, cnt) : 0;
-  if (tid < 64) finish_row(A, r, t, L);
+  First first;
+  if (tid < 64) first = row_state(A, r, t, L);
   if (tid == 0) L.scale = scale_of(A, r, counted);
   __syncthreads();
   T* out = (T*)A.dlogits + A.out_at.offset(r);
   if (L.st.ok == 0.f || !same_granules(row.p, (const T*)out)) {   // (a gradient that lies otherwise in its granules)
     grad_of_segment<T, G, 1>(A, row, r, 0, row.nq, L);
+    if (tid < 64) row_loss(A, r, first, L);
     return;
   }
   const Dense dn(A, L.st, L.scale);
@@ -1275,6 +1333,7 @@ __global__ __launch_bounds__(G) void distill_held_kernel(DistillArgs A) {
   else put([&](float z) { return dn.one(z); });
   barrier_after_stores();   // the entries are written over the dense values
   put_entries<T, G>(A, row, r, out, 0, row.V, dn, L, L.scale);
+  if (tid < 64) row_loss(A, r, first, L);   // behind the gradient: its registers are free, and nothing waits for it
 }
 
 // the gradient alone, from the state that the loss left
@@ -1338,6 +1397,12 @@ Plan plan_rows(int R, int nq) {
     if (nq <= 64 * nv) return {64, nv};
   return {nq <= 2048 || R > vitm_cu_count() ? 256 : 1024, 4};
 }
+// Whether the sums over a row leave the teacher's classes out: the tail form, which asks for the mass outside the list, and
+// temperatures above kFlat.  Left in, they leave the loss off by what ln s is off by, 1e-7 or so, times T^2 (2e-6 of a loss of 4 at
+// T = 8, and growing); taken out, 4e-7 up to T = 10^4, but loss and gradient of 4096 x 32000 bf16 take 136 us against 108 us,
+// 8192 x 1000 fp32 39 against 33.
+constexpr float kFlat = 8.f;
+int keeps_apart(int tail, float temperature) { return tail || temperature > kFlat; }
 // Threads, chunk, and the cut of a row for kernels whose segments do not depend on each other.
 constexpr int kMapSpan = 2048;   // most granules of a segment: 94 us without a limit, 70 us with, at 1024 x 50001 fp32
 struct Cut {
@@ -1396,10 +1461,11 @@ bool rows_meet(const void* logits, const void* out, int dtype, const RowsAt& at,
   }
   return false;
 }
-constexpr float kMinTemperature = 1e-6f, kMaxTemperature = 1e6f;
-int check_temperature(const char* what, float t) {
-  VITM_REQUIRE(t >= kMinTemperature && t <= kMaxTemperature, "%s: temperature %g, supported are %g to %g", what, (double)t,
-               (double)kMinTemperature, (double)kMaxTemperature);
+// The gradient of a distillation, T (p - q), is off by what ln s is off by, times T: by 3e-3 of itself at T = 10^4 (V = 40001).
+constexpr float kMinTemperature = 1e-6f, kMaxTemperature = 1e6f, kMaxDistillTemperature = 1e4f;
+int check_temperature(const char* what, float t, float most = kMaxTemperature) {
+  VITM_REQUIRE(t >= kMinTemperature && t <= most, "%s: temperature %g, supported are %g to %g", what, (double)t,
+               (double)kMinTemperature, (double)most);
   return VITM_OK;
 }
 // a grid holds fewer than 2^32 threads
@@ -1453,7 +1519,7 @@ template <typename T> void launch_log_probs_bwd(const LogProbsBwdArgs& A, const 
 }
 constexpr int kMarks = 131072;   // most granules of a row: the marks of the tail form
 template <typename T, bool GRAD> int launch_distill_rows(const DistillArgs& A, const Plan& P, int nq, hipStream_t st) {
-  const int lds = A.tail ? cover(nq, 4) * 4 : 0;
+  const int lds = A.apart ? cover(nq, 4) * 4 : 0;
 #define DS(G, NV)                                                                                                       \
   if (lds > 32768) VITM_LDS_OPTIN((distill_rows_kernel<T, G, NV, GRAD>), kMarks, "vitm_distill");                       \
   SCORES_LAUNCH((distill_rows_kernel<T, G, NV, GRAD>), A.R, G, lds, A)
@@ -1470,8 +1536,8 @@ template <typename T, bool GRAD> int launch_distill_rows(const DistillArgs& A, c
 // no classes have to be taken out of the sums (4096 x 32000 bf16: 117 us against 135 us with a second reading; 2048 x 32000 fp32:
 // 106 against 131); with the tail's marks the walk is the faster one (4096 x 50001 bf16: 211 us against 253 us held).  A row of
 // 16384 granules fills the registers of a CU, and nothing runs beside its phases: 640 us against 500 us at 4096 x 131072 bf16.
-Plan plan_distill_fused(int R, int nq, bool tail) {   // NV = 0: a walk by launch_distill_rows
-  if (nq <= 1024 || (!tail && nq <= 8192)) {
+Plan plan_distill_fused(int R, int nq, bool apart) {   // NV = 0: a walk by launch_distill_rows
+  if (nq <= 1024 || (!apart && nq <= 8192)) {
     if (nq <= 256) return {64, nq <= 64 ? 1 : nq <= 128 ? 2 : 4};
     if (nq <= 4096) return {256, nq <= 1024 ? 4 : nq <= 2048 ? 8 : 16};
     return {512, 16};
@@ -1480,7 +1546,7 @@ Plan plan_distill_fused(int R, int nq, bool tail) {   // NV = 0: a walk by launc
 }
 template <typename T> int launch_distill_fused(const DistillArgs& A, const Plan& P, int nq, hipStream_t st) {
   if (P.NV == 0) return launch_distill_rows<T, true>(A, P, nq, st);
-  const int lds = A.tail ? cover(nq, 4) * 4 : 0;
+  const int lds = A.apart ? cover(nq, 4) * 4 : 0;
 #define DH(G, NV) SCORES_LAUNCH((distill_held_kernel<T, G, NV>), A.R, G, lds, A)
   if (P.G == 64 && P.NV == 1) DH(64, 1);
   else if (P.G == 64 && P.NV == 2) DH(64, 2);
@@ -1580,7 +1646,7 @@ int distill_args(const char* what, DistillArgs& A, const void* logits, int dtype
                  const int64_t* labels, int64_t ignore_index) {
   const int rc = check_rows(what, logits, dtype, ld_outer, ld, inner, R, V);
   if (rc != VITM_OK) return rc;
-  if (check_temperature(what, temperature) != VITM_OK) return VITM_EINVAL;
+  if (check_temperature(what, temperature, kMaxDistillTemperature) != VITM_OK) return VITM_EINVAL;
   VITM_REQUIRE(label_weight >= 0.f && label_weight <= 1.f, "%s: label weight must lie in [0, 1]", what);
   VITM_REQUIRE(label_weight == 0.f || labels, "%s: a label weight needs labels", what);
   VITM_REQUIRE(teacher && indices, "%s: null pointer", what);
@@ -1589,6 +1655,7 @@ int distill_args(const char* what, DistillArgs& A, const void* logits, int dtype
   A.at = {ld_outer, ld, inner};
   A.R = R; A.V = V;
   A.temperature = temperature; A.label_weight = label_weight; A.tail = tail ? 1 : 0;
+  A.apart = keeps_apart(A.tail, temperature);
   A.teacher = teacher; A.indices = indices; A.K = K;
   A.labels = labels; A.ignore = ignore_index;
   A.host_scale = 1.f;
@@ -1616,7 +1683,7 @@ extern "C" int vitm_distill(const void* logits, int dtype, int64_t ld_outer, int
                  "vitm_distill: logits and gradient in the same memory");
   }
   const int nq = row_granules(dtype, V, slack_of(logits, dtype, ld_outer, ld, inner, R));
-  const Plan P = dlogits ? plan_distill_fused(R, nq, tail != 0) : plan_rows(R, nq);
+  const Plan P = dlogits ? plan_distill_fused(R, nq, A.apart) : plan_rows(R, nq);
   if (check_grid("vitm_distill", R, R, P.G) != VITM_OK) return VITM_EINVAL;
   A.row_loss = row_loss;
   A.state = state;

@@ -18,6 +18,7 @@ BF16, F32 = 0, 1
 STATS_PARTS = 4   # VITM_STATS_PARTS
 ACT_GELU_ERF, ACT_RELU, ACT_GELU_TANH, ACT_SILU, ACT_SIGMOID, ACT_TANH = range(6)   # enum vitm_activation_kind
 SCORES_MAX_CLASSES, SCORES_MAX_TOP, DISTILL_STATE = 500000, 128, 8   # vitm_scores_max_classes() ..., vitm_distill_state_floats()
+SCORES_MAX_TEMPERATURE, DISTILL_MAX_TEMPERATURE = 1e6, 1e4
 SCORES_MAX_ROWS = 1 << 30            # the C ABI counts rows in an int; one launch may hold fewer of them (it says so)
 REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = range(3)                                      # enum vitm_reduction
 EPI_BIAS, EPI_BIAS_GELU, EPI_LN, EPI_LN_GELU, EPI_RESIDUAL, EPI_DGELU, EPI_BIAS_GELU2 = 0, 1, 2, 3, 4, 5, 6

@@ -22,7 +22,7 @@ class LogProbs(NamedTuple):
     top_indices: Optional[torch.Tensor]
 
 
-def check_scores(logits: torch.Tensor, temperature: float, what: str) -> None:
+def check_scores(logits: torch.Tensor, temperature: float, what: str, most: float = _lib.SCORES_MAX_TEMPERATURE) -> None:
     """The checks every operator on class scores shares."""
     if logits.dim() < 1:
         raise ValueError(f"{what}: logits need a class dimension")
@@ -32,7 +32,7 @@ def check_scores(logits: torch.Tensor, temperature: float, what: str) -> None:
         raise ValueError(f"{what}: {logits.shape[-1]} classes, supported are 1 to {_lib.SCORES_MAX_CLASSES}")
     if logits.numel() > _lib.SCORES_MAX_ROWS * logits.shape[-1]:
         raise ValueError(f"{what}: {logits.numel() // logits.shape[-1]} rows, supported are at most {_lib.SCORES_MAX_ROWS}")
-    check_temperature(temperature, what)
+    check_temperature(temperature, what, most)
     refuse_tangents(what, logits)
 
 
@@ -43,9 +43,9 @@ def refuse_tangents(what: str, *inputs: torch.Tensor) -> None:
             raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
-def check_temperature(temperature: float, what: str) -> None:
-    if not 1e-6 <= temperature <= 1e6:
-        raise ValueError(f"{what}: temperature {temperature}, supported are 1e-6 to 1e6")
+def check_temperature(temperature: float, what: str, most: float = _lib.SCORES_MAX_TEMPERATURE) -> None:
+    if not 1e-6 <= temperature <= most:
+        raise ValueError(f"{what}: temperature {temperature}, supported are 1e-6 to {most:g}")
 
 
 def check_indices(t: torch.Tensor, logits: torch.Tensor, what: str) -> None:

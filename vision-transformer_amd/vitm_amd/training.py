@@ -580,6 +580,10 @@ class DistillationLoss(nn.Module):
     ``label_weight=0``).  A label or an index outside the classes gives the row a NaN loss and a zero gradient.  Masked
     (-inf) classes are allowed; a row that has only such has loss and gradient 0.
 
+    Temperatures lie in [1e-6, 1e4].  A loss is T^2 times a divergence that shrinks with T^2, a gradient T times a difference
+    that shrinks with T: up to T = 8 the loss is good to about T^2 * 1e-7, beyond (and with ``tail=True``) to T * 1e-7 of
+    itself, the gradient to T * 3e-7 of itself.
+
     ``forward`` is differentiable with respect to the logits (bf16 or fp32, (..., V)); ``loss_and_grad`` reads them once and
     returns loss and gradient without an autograd graph (what ``Trainer`` and a captured step use)."""
 
@@ -590,7 +594,7 @@ class DistillationLoss(nn.Module):
             raise ValueError(f"DistillationLoss: label_weight {label_weight} outside [0, 1]")
         if reduction not in score_ops.REDUCTIONS:
             raise ValueError(f"DistillationLoss: reduction {reduction!r}, supported are {sorted(score_ops.REDUCTIONS)}")
-        scores.check_temperature(temperature, "DistillationLoss")
+        scores.check_temperature(temperature, "DistillationLoss", _lib.DISTILL_MAX_TEMPERATURE)
         self.temperature, self.label_weight, self.tail = float(temperature), float(label_weight), bool(tail)
         self.reduction, self.ignore_index = reduction, int(ignore_index)
 
@@ -600,7 +604,7 @@ class DistillationLoss(nn.Module):
 
     def _checked(self, logits, teacher, indices, labels, tracked):
         what = "DistillationLoss"
-        scores.check_scores(logits, self.temperature, what)
+        scores.check_scores(logits, self.temperature, what, _lib.DISTILL_MAX_TEMPERATURE)
         lead = logits.shape[:-1]
         most = _lib.SCORES_MAX_TOP
         if teacher.shape[:-1] != lead or teacher.dim() != logits.dim() or not 1 <= teacher.shape[-1] <= most:
