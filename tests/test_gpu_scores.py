@@ -786,3 +786,57 @@ def test_distillation_at_high_temperatures(log_probs, Loss, R, V, K, tail, kind,
     _near(l2.detach(), ref, T ** 2 * kl_tol, "loss")
     (d2,) = torch.autograd.grad(l2, zr, torch.ones(R, device=DEV))
     _check_distill(z, tl, idx, None, None, d2, T, 0.0, tail)
+
+
+@pytest.mark.parametrize("R", [1023, 1024, 1025, 2049, 4100])
+@pytest.mark.parametrize("V,tail", [(7, False), (300, True)])
+def test_distillation_of_many_rows(Loss, R, V, tail):
+    """On both sides of 1024 rows: up to there every workgroup counts the labels itself, beyond a kernel counts them first, in
+    rounds of 1024, and the total adds several rows a thread.  Ignored labels lie in every round, so that a round left out or
+    counted twice shows."""
+    T, a, K = 2.0, 0.4, 3
+    z = _scores(R, V, F32, R)
+    idx = torch.stack([torch.randperm(V, generator=_gen(i % 64))[:K] for i in range(R)]).to(DEV)
+    tl = torch.log_softmax(torch.randn(R, K + 1, generator=_gen(R)), 1)[:, :K].to(DEV)
+    labels = torch.randint(0, V, (R,), generator=_gen(1))
+    labels[torch.rand(R, generator=_gen(2)) < torch.arange(R) / R] = -100      # few at first, most at the end
+    labels = labels.to(DEV)
+    n = int((labels != -100).sum())
+    each = Loss(T, a, tail, "none")(z, tl, idx, labels)
+    ref, mag, c = _check_distill(z, tl, idx, labels, each, None, T, a, tail)
+    for red, div in (("mean", n), ("sum", 1)):
+        up = torch.full((R,), 1.0 / div, device=DEV)
+        want = each.double().sum() / div
+        loss, dz = Loss(T, a, tail, red).loss_and_grad(z, tl, idx, labels)
+        _near(loss, want, 2 * U * (c * mag).sum() / div + U * want.abs(), red)   # its rows' sums may be taken in another order
+        _check_distill(z, tl, idx, labels, None, dz, T, a, tail, up)
+        zr = z.clone().requires_grad_(True)
+        l2 = Loss(T, a, tail, red)(zr, tl, idx, labels)
+        assert torch.equal(l2.detach(), Loss(T, a, tail, red)(z, tl, idx, labels))
+        (d2,) = torch.autograd.grad(l2, zr)
+        _check_distill(z, tl, idx, labels, None, d2, T, a, tail, up)
+    loss, dz = Loss(T, a, tail).loss_and_grad(z, tl, idx, torch.full_like(labels, -100))
+    assert loss == 0 and (dz == 0).all()
+
+
+@pytest.mark.parametrize("R,V,dtype", [(1500, 300, BF), (2100, 33, F32)])
+def test_many_rows_captured(log_probs, Loss, R, V, dtype):
+    """The count of the rows in memory, from a graph replayed several times between eager work."""
+    z = _scores(R, V, dtype, 2)
+    idx = torch.stack([torch.randperm(V, generator=_gen(i % 50))[:9] for i in range(R)]).to(DEV)
+    tl = torch.log_softmax(torch.randn(R, 10, generator=_gen(9)), 1)[:, :9].to(DEV)
+    tgt = torch.randint(0, V, (R,), generator=_gen(2)).to(DEV)
+    fn = _calls(log_probs, Loss, z, tl, idx, tgt)
+    first = fn()
+    assert all(torch.equal(a, b) for a, b in zip(first, fn()))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fn()
+    for step in range(4):
+        z.copy_(_scores(R, V, dtype, 20 + step))
+        tgt[step::7] = -100                       # another count each time
+        graph.replay()
+        eager = fn()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager)), step
