@@ -29,7 +29,7 @@ def graphed(monkeypatch):
         tr = SimpleNamespace(params=object(), reducer=SimpleNamespace(active=False), optimizer=_Optimizer(), scheduler=None,
                              distillation=loss or training.DistillationLoss(), teacher=teacher, teacher_top_k=4,
                              step=lambda *a: torch.zeros(()),
-                             device_step=lambda x, y, hyper, top: (torch.zeros(()), torch.zeros(())))
+                             device_step=lambda x, y, hyper, top=None: (torch.zeros(()), torch.zeros(())))
         g = GraphedTrainStep(tr, warmup=1)
         x, y = torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64)
         step = lambda: g.step(x, y, top)
@@ -124,7 +124,7 @@ def test_captured_step_keeps_what_its_kernels_read(graphed):
     from vitm_amd import GraphedTrainStep
     g, tr, step = graphed(m)
     capture = GraphedTrainStep._capture
-    tr.device_step = lambda x, y, hyper, top: (_ops.cached_pack(owner, "w", (m[0].weight,), build).__class__ and torch.zeros(()),
+    tr.device_step = lambda x, y, hyper: (_ops.cached_pack(owner, "w", (m[0].weight,), build).__class__ and torch.zeros(()),
                                                _ops.f32vec(half))
     capture(g, torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64), None)
     vec = weakref.ref(half._vitm_f32[1])
@@ -170,3 +170,14 @@ def test_a_capture_that_failed_is_not_replayed(graphed):
     assert g.graph is None and tr.optimizer.steps == 2
     g.step(*args)
     assert g.graph is not None and tr.optimizer.steps == 3
+
+
+def test_captured_step_of_a_trainer_without_distillation(graphed, monkeypatch):
+    """A trainer of the caller's own, or a subclass, whose steps take images and labels only."""
+    from vitm_amd import GraphedTrainStep
+    tr = SimpleNamespace(params=object(), reducer=SimpleNamespace(active=False), optimizer=_Optimizer(), scheduler=None,
+                         step=lambda images, labels: torch.zeros(()), device_step=lambda images, labels, hyper: (torch.zeros(()), torch.zeros(())))
+    g = GraphedTrainStep(tr, warmup=1)
+    for _ in range(3):
+        g.step(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64))
+    assert tr.optimizer.steps == 2

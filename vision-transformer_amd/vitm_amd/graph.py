@@ -76,7 +76,7 @@ class GraphedTrainStep:
         """(settings of the loss, what the captured teacher's weights were made from): the latter is what packed weights are
         kept by; buffers are read where they are, so only their place counts."""
         tr = self.trainer
-        if tr.distillation is None:
+        if getattr(tr, "distillation", None) is None:
             return None, None
         t = tr.teacher
         if self.top is not None:
@@ -96,20 +96,21 @@ class GraphedTrainStep:
         self.distilled_from = self._distilled_from()
         # what the graph's kernels read has to outlive whatever becomes of the teacher
         self.held = []
-        if self.top is None and isinstance(tr.teacher, torch.nn.Module):
-            self.held += [t.detach() for t in (*tr.teacher.parameters(), *tr.teacher.buffers())]
+        teacher = getattr(tr, "teacher", None)
+        if self.top is None and isinstance(teacher, torch.nn.Module):
+            self.held += [t.detach() for t in (*teacher.parameters(), *teacher.buffers())]
         self.hyper = torch.zeros(8, dtype=torch.float32, device=dev)
         torch.cuda.synchronize(dev)
         graph = torch.cuda.CUDAGraph()
         with _ops.holding(self.held), torch.cuda.graph(graph):
-            self.loss, self.norm = tr.device_step(self.x, self.y, self.hyper, self.top)
+            self.loss, self.norm = tr.device_step(self.x, self.y, self.hyper, *(() if self.top is None else (self.top,)))
         self.graph = graph
 
     def step(self, images: torch.Tensor, labels: torch.Tensor, teacher_top=None) -> torch.Tensor:
         tr = self.trainer
         self.calls += 1
         if self.calls <= self.warmup:
-            return tr.step(images, labels, teacher_top)
+            return tr.step(images, labels, *(() if teacher_top is None else (teacher_top,)))
         if self.graph is None:
             self._capture(images, labels, teacher_top)
         if images.shape != self.x.shape or images.dtype != self.x.dtype or labels.shape != self.y.shape:
