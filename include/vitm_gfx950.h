@@ -437,8 +437,8 @@ int vitm_log_probs(const void* logits, int dtype, int64_t ld_outer, int64_t ld, 
 /*
  * Gradient of vitm_log_probs: dlogits (in `dtype`, rows at ldd_outer / ldd) from the gradients of its outputs, each of
  * which may be null (0): g_logprobs [R, n_targets], g_lse [R], g_entropy [R] (needs `entropy`), g_top [R, top_k] (needs
- * `top_indices`).  A class that occurs several times among targets and top classes gets the sum.  dlogits must not overlap
- * logits.
+ * `top_indices`).  A class that occurs several times among targets and top classes gets the sum.  A dlogits whose rows
+ * meet those of logits is refused.
  */
 int vitm_log_probs_bwd(const void* logits, int dtype, int64_t ld_outer, int64_t ld, int inner, int R, int V,
                        float temperature, const int64_t* targets, int n_targets, int64_t ignore_index,
@@ -457,7 +457,7 @@ int vitm_log_probs_bwd(const void* logits, int dtype, int64_t ld_outer, int64_t 
  * bounds.  `loss` (one float) is the sum of the rows (VITM_REDUCE_SUM) or that over the number of counted rows
  * (VITM_REDUCE_MEAN; inv_count, one float, receives its reciprocal where labels are given).
  * dlogits (nullable): the gradient of `loss` (of every row's loss with VITM_REDUCE_NONE), in the same pass over the logits for
- * rows of up to 8192 16-byte pieces (tail = 0; 1024 with it).  It must not overlap logits.  state (nullable,
+ * rows of up to 8192 16-byte pieces (1024 with a tail, or T > 8).  Rows that meet those of logits are refused.  state (nullable,
  * vitm_distill_state_floats() floats a row): what vitm_distill_bwd needs.
  */
 int vitm_distill_state_floats(void);

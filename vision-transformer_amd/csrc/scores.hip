@@ -8,16 +8,16 @@
 //                   (1 - a) T^2 [sum q_k (ln q_k - ln p(c_k)) + q_r (ln q_r - ln p_r)] + a CE(z, y), and d/dz
 //
 // All of them are bound by HBM: one multiply-add, one exponential and a few adds per class against 2 or 4 bytes.  A row belongs
-// to one wave or workgroup (plan_rows) that walks over it in 16-byte granules with running maxima and sums (5.9 TB/s of reads at
-// 4096 x 65537 bf16 with entropies, where a copy of 2 GiB reaches 4.9 TB/s of reads and writes); what belongs to the row besides,
-// the given classes, the top list, the teacher's list, hides behind other rows' walks.  Loss and gradient in one call keep the
-// row in registers between the two where that is faster (launch_distill_fused).  Classes that pass once bypass the caches
+// to one wave or workgroup (plan_rows) that walks over it in 16-byte granules with running maxima and sums (6.0 TB/s of reads at
+// 4096 x 65537 bf16 with entropies, call after call, 5.6 under the profiler, where a copy of 2 GiB reaches 4.9 TB/s of reads and
+// writes); what belongs to the row besides, the given classes, the top list, the teacher's list, hides behind other rows' walks.
+// Loss and gradient in one call keep the row in registers between the two where that is faster (plan_distill_fused).  Classes that pass once bypass the caches
 // (nontemporal): 81 us against 95 us for the bare walk over 512 MiB.
 // A granule is 16 aligned bytes of memory, whatever the alignment of the row: the granules a row covers only in part are read and
 // written class by class, so that nothing outside the row is touched and odd row lengths keep 16-byte accesses.
 //
-// Sums and maxima are fp32, combined in a fixed order; no floating-point atomics, so equal calls give equal bits.  Outputs of 16
-// bits are rounded once, from fp32.
+// Sums and maxima are fp32, combined in a fixed order (of a distillation's logarithms, their differences and the rows' total: 64
+// bits); no floating-point atomics, so equal calls give equal bits.  Outputs of 16 bits are rounded once, from fp32.
 #include "common.h"
 
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4_t;
@@ -1533,8 +1533,9 @@ template <typename T, bool GRAD> int launch_distill_rows(const DistillArgs& A, c
   return VITM_OK;
 }
 // Loss and gradient in one kernel.  Rows of up to 1024 granules stay in registers.  Longer ones do too, up to 8192 granules, where
-// no classes have to be taken out of the sums (4096 x 32000 bf16: 117 us against 135 us with a second reading; 2048 x 32000 fp32:
-// 106 against 131); with the tail's marks the walk is the faster one (4096 x 50001 bf16: 211 us against 253 us held).  A row of
+// no classes have to be taken out of the sums (4096 x 32000 bf16: 110 us against 135 us with a second reading; 2048 x 32000 fp32:
+// 105 against 128); with the marks of the listed classes the walk is the faster one for long lists (4096 x 50001 bf16: 222 us
+// against 246 us held with 64 entries, 248 against 344 with 128, 211 against 203 with 20).  A row of
 // 16384 granules fills the registers of a CU, and nothing runs beside its phases: 640 us against 500 us at 4096 x 131072 bf16.
 Plan plan_distill_fused(int R, int nq, bool apart) {   // NV = 0: a walk by launch_distill_rows
   if (nq <= 1024 || (!apart && nq <= 8192)) {
