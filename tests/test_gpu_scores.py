@@ -840,3 +840,19 @@ def test_many_rows_captured(log_probs, Loss, R, V, dtype):
         eager = fn()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, eager)), step
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("top_k", [0, 1])
+@pytest.mark.parametrize("z0", [0.0, -3.0])
+def test_logarithms_of_exact_sums(log_probs, dtype, top_k, z0):
+    """V equal classes: every exponential is 1 and their sum V exactly, so that lse = z0 + ln V, log p = -ln V and the entropy
+    ln V are off by the logarithm (its hardware form good to 2^-24 in [0.5, 1), times ln 2 that is off by 2^-25 of it: 2^-24 in all)
+    and the final rounding alone."""
+    for V in [2, 3, 5, 7, 10, 11, 13, 37, 100, 101, 997, 1000, 1001, 3001, 4093, 10007, 21001, 50021, 99991, 131071, 300007]:
+        r = log_probs(torch.full((2, V), z0, device=DEV, dtype=dtype), torch.zeros(2, dtype=torch.int64, device=DEV), top_k=top_k,
+                      entropy=True)
+        ln = torch.log(torch.tensor(float(V), dtype=torch.float64, device=DEV))
+        for got, want in ((r.lse, z0 + ln), (r.logprobs, -ln), (r.entropy, ln), (r.top_logprobs, -ln)):
+            if got is not None:
+                assert ((got.double() - want).abs() <= U * want.abs() + U).all(), (V, got, want)

@@ -16,8 +16,8 @@
 // A granule is 16 aligned bytes of memory, whatever the alignment of the row: the granules a row covers only in part are read and
 // written class by class, so that nothing outside the row is touched and odd row lengths keep 16-byte accesses.
 //
-// Sums and maxima are fp32, combined in a fixed order (of a distillation's logarithms, their differences and the rows' total: 64
-// bits); no floating-point atomics, so equal calls give equal bits.  Outputs of 16 bits are rounded once, from fp32.
+// Sums and maxima are fp32, combined in a fixed order (logarithms and their differences, and the total of a distillation's
+// rows: 64 bits); no floating-point atomics, so equal calls give equal bits.  Outputs of 16 bits are rounded once, from fp32.
 #include "common.h"
 
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4_t;
@@ -614,14 +614,18 @@ template <typename T> __device__ __forceinline__ Given fetch_given(const LogProb
   }
   return v;
 }
+// x - lse for a score z: the difference is 64 bits and rounded once
+__device__ __forceinline__ float log_prob(const LogProbsArgs& A, float z, float m, double ln_s) {
+  return (float)fma((double)z - (double)m, (double)A.inv_t, -ln_s);
+}
 // everything of a row that follows from its sums, by `n` threads, each of which holds the given class of its own number
 template <typename T>
 __device__ __forceinline__ void row_answers(const LogProbsArgs& A, const T* p, int r, Sums t, Given v, int tid, int n) {
-  const float ln_s = ln_of(t.s);
+  const double ln_s = wide_ln_of(t.s);
   const bool none = t.m == NINF && t.s == 0.f;      // no class has a finite score
   if (tid == 0) {
-    if (A.lse) A.lse[r] = none ? NINF : fmaf(t.m, A.inv_t, ln_s);
-    if (A.entropy) A.entropy[r] = none ? 0.f : ln_s - kLn2 * (t.u / t.s);
+    if (A.lse) A.lse[r] = none ? NINF : (float)fma((double)t.m, (double)A.inv_t, ln_s);
+    if (A.entropy) A.entropy[r] = none ? 0.f : (float)(ln_s - (double)(kLn2 * (t.u / t.s)));
     if (A.stats) {
       A.stats[2 * (int64_t)r] = t.m;
       A.stats[2 * (int64_t)r + 1] = t.s;
@@ -632,24 +636,24 @@ __device__ __forceinline__ void row_answers(const LogProbsArgs& A, const T* p, i
     float lp = 0.f;
     if (v.y != A.ignore) {
       if (v.y < 0 || v.y >= A.V) lp = __builtin_nanf("");
-      else lp = none ? NINF : (v.z - t.m) * A.inv_t - ln_s;
+      else lp = none ? NINF : log_prob(A, v.z, t.m, ln_s);
     }
     A.logprobs[(int64_t)r * A.G + g] = lp;
   }
 }
 __device__ __forceinline__ void put_list(const LogProbsArgs& A, int r, Sums t, const TopList& L, int tid, int n) {
-  const float ln_s = ln_of(t.s);
+  const double ln_s = wide_ln_of(t.s);
   const bool nan = t.s != t.s;
   for (int k = tid; k < A.K; k += n) {
     const int64_t at = (int64_t)r * A.K + k;
     const key64 v = L.key[L.cur][k];
-    A.top_lp[at] = nan ? t.s : t.m == NINF ? NINF : (value_of(v) - t.m) * A.inv_t - ln_s;
+    A.top_lp[at] = nan ? t.s : t.m == NINF ? NINF : log_prob(A, value_of(v), t.m, ln_s);
     A.top_idx[at] = nan ? -1 : (int64_t)class_of(v);
   }
 }
 
 // Short rows share a workgroup of 256 threads, the shortest a wave: 4 lanes a row of up to 4 granules, 16 up to 16.  A million
-// rows of 10 bf16 classes take 440 us with a wave each, bound by instructions, 35 us so.
+// rows of 10 bf16 classes with a target each take 440 us with a wave each, bound by instructions, 37 us so.
 constexpr int rows_of_group(int G) { return G <= 64 ? 256 / G : 1; }
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(G * rows_of_group(G)) void log_probs_kernel(LogProbsArgs A) {
@@ -853,7 +857,7 @@ __global__ __launch_bounds__(G) void log_probs_bwd_kernel(LogProbsBwdArgs A) {
   const float lead = (A.g_lse ? A.g_lse[r] : 0.f) - s_sum;
   // dz = w (k0 - k1 t) with w = 2^t, t = c (z - m): log p + H = ln2 t - ln s + H
   const float scale = none ? 0.f : A.inv_t / s;
-  const float k1 = gh * kLn2, k0 = lead - (A.g_entropy ? gh * (A.entropy[r] - ln_of(s)) : 0.f);
+  const float k1 = gh * kLn2, k0 = lead - (A.g_entropy ? gh * (float)((double)A.entropy[r] - wide_ln_of(s)) : 0.f);
   auto dense = [&](float z) {
     const float t = (z - m) * c, w = __builtin_amdgcn_exp2f(t) * scale;
     return none || w == 0.f ? 0.f : w * fmaf(-k1, t, k0);
@@ -1384,7 +1388,7 @@ int cover(int a, int b) { return (a + b - 1) / b; }
 int row_granules(int dtype, int V, int slack) { return cover(V + slack, granule_classes(dtype)); }
 
 // Threads a row, and granules a thread and chunk.  One wave takes a row of up to 256 granules (2048 bf16 classes): 16384 rows of
-// 2000 take 16 us so, 45 us with 256 threads each.  Longer rows have a workgroup of 256 threads (2048 rows of 32001: 28 us, with
+// 2000 take 17 us so, 45 us with 256 threads each.  Longer rows have a workgroup of 256 threads (2048 rows of 32001: 28 us, with
 // 1024 threads 31 us), or, where there are no more rows than CUs, of 1024 from 2048 granules on (64 rows with 20 best: 16384 classes
 // 8.5 us with 256 threads and 10.4 us with 1024; 65536 classes 18.7 and 14.1 us).  A row is never cut: one row of 131072 classes
 // with 20 best takes one workgroup 16 us, 10 of them for the arithmetic; cut into 64 segments and joined it took 23 us in two
