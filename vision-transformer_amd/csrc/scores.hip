@@ -615,16 +615,18 @@ template <typename T> __device__ __forceinline__ Given fetch_given(const LogProb
   return v;
 }
 // x - lse for a score z: the difference is 64 bits and rounded once
-__device__ __forceinline__ float log_prob(const LogProbsArgs& A, float z, float m, double ln_s) {
-  return (float)fma((double)z - (double)m, (double)A.inv_t, -ln_s);
+__device__ __forceinline__ float log_prob(float z, float m, float inv_t, double ln_s) {
+  return (float)fma((double)z - (double)m, (double)inv_t, -ln_s);
 }
 // everything of a row that follows from its sums, by `n` threads, each of which holds the given class of its own number
 template <typename T>
 __device__ __forceinline__ void row_answers(const LogProbsArgs& A, const T* p, int r, Sums t, Given v, int tid, int n) {
+  float inv_t = A.inv_t;
+  asm volatile("" : "+v"(inv_t), "+v"(v.z));   // widened here: in front of the walk the 64 bits would cost it registers
   const double ln_s = wide_ln_of(t.s);
   const bool none = t.m == NINF && t.s == 0.f;      // no class has a finite score
   if (tid == 0) {
-    if (A.lse) A.lse[r] = none ? NINF : (float)fma((double)t.m, (double)A.inv_t, ln_s);
+    if (A.lse) A.lse[r] = none ? NINF : (float)fma((double)t.m, (double)inv_t, ln_s);
     if (A.entropy) A.entropy[r] = none ? 0.f : (float)(ln_s - (double)(kLn2 * (t.u / t.s)));
     if (A.stats) {
       A.stats[2 * (int64_t)r] = t.m;
@@ -636,7 +638,7 @@ __device__ __forceinline__ void row_answers(const LogProbsArgs& A, const T* p, i
     float lp = 0.f;
     if (v.y != A.ignore) {
       if (v.y < 0 || v.y >= A.V) lp = __builtin_nanf("");
-      else lp = none ? NINF : log_prob(A, v.z, t.m, ln_s);
+      else lp = none ? NINF : log_prob(v.z, t.m, inv_t, ln_s);
     }
     A.logprobs[(int64_t)r * A.G + g] = lp;
   }
@@ -647,13 +649,13 @@ __device__ __forceinline__ void put_list(const LogProbsArgs& A, int r, Sums t, c
   for (int k = tid; k < A.K; k += n) {
     const int64_t at = (int64_t)r * A.K + k;
     const key64 v = L.key[L.cur][k];
-    A.top_lp[at] = nan ? t.s : t.m == NINF ? NINF : log_prob(A, value_of(v), t.m, ln_s);
+    A.top_lp[at] = nan ? t.s : t.m == NINF ? NINF : log_prob(value_of(v), t.m, A.inv_t, ln_s);
     A.top_idx[at] = nan ? -1 : (int64_t)class_of(v);
   }
 }
 
 // Short rows share a workgroup of 256 threads, the shortest a wave: 4 lanes a row of up to 4 granules, 16 up to 16.  A million
-// rows of 10 bf16 classes with a target each take 440 us with a wave each, bound by instructions, 37 us so.
+// rows of 10 bf16 classes with a target each take 440 us with a wave each, bound by instructions, 36 us so.
 constexpr int rows_of_group(int G) { return G <= 64 ? 256 / G : 1; }
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(G * rows_of_group(G)) void log_probs_kernel(LogProbsArgs A) {
@@ -1388,7 +1390,7 @@ int cover(int a, int b) { return (a + b - 1) / b; }
 int row_granules(int dtype, int V, int slack) { return cover(V + slack, granule_classes(dtype)); }
 
 // Threads a row, and granules a thread and chunk.  One wave takes a row of up to 256 granules (2048 bf16 classes): 16384 rows of
-// 2000 take 17 us so, 45 us with 256 threads each.  Longer rows have a workgroup of 256 threads (2048 rows of 32001: 28 us, with
+// 2000 take 16 us so, 45 us with 256 threads each.  Longer rows have a workgroup of 256 threads (2048 rows of 32001: 28 us, with
 // 1024 threads 31 us), or, where there are no more rows than CUs, of 1024 from 2048 granules on (64 rows with 20 best: 16384 classes
 // 8.5 us with 256 threads and 10.4 us with 1024; 65536 classes 18.7 and 14.1 us).  A row is never cut: one row of 131072 classes
 // with 20 best takes one workgroup 16 us, 10 of them for the arithmetic; cut into 64 segments and joined it took 23 us in two
