@@ -62,8 +62,8 @@ class GraphedTrainStep:
 
     A teacher of the trainer's is captured with the step, its weights as they are then.  A module whose parameters were
     written in place, moved, cast or replaced since is refused (hand ``step`` the ``teacher_top`` of such a teacher), and so
-    are another teacher and other settings of the distillation loss.  A write through ``p.data`` leaves no trace that could
-    be looked at and goes unseen; a teacher that is no module has to stay what it was.
+    are another teacher and other settings of the distillation loss.  An in-place write through ``p.data`` leaves no trace
+    that could be looked at and goes unseen; a teacher that is no module has to stay what it was.
     """
 
     def __init__(self, trainer, warmup: int = 2):
